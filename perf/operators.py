@@ -16,7 +16,7 @@ own = False
 
 DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16}
 ELEM = {"float32": 4, "bfloat16": 2}
-TINY = 2.0 ** -126  # smallest normal float32: smaller scales are taken as zero
+TINY = 2.0 ** -100  # smaller scales are taken as zero
 
 
 # ------------------------------------------------------------------------------------- cases
