@@ -56,6 +56,7 @@ typedef enum vfl_dtype {
                                      the table; the length was clamped                      */
 #define VFL_DEVERR_TIMEOUT 0x8u   /* a bounded wait on a shared-memory barrier gave up      */
 #define VFL_DEVERR_QUERY 0x10u    /* query_start_loc not non-decreasing / beyond num_tokens  */
+#define VFL_DEVERR_NONFINITE 0x20u /* an infinity or NaN was stored in an 8-bit cache         */
 
 /* How a plan spreads the work over CTAs.
  * VFL_SCHEDULE_ITEMS: one CTA per (request, head group, query chunk, split-K range).
@@ -352,6 +353,100 @@ int vfl_beam_merge(const float* values, const int32_t* indices, int64_t rows, in
  *   or a position past width are skipped and flagged with VFL_DEVERR_SLOT. */
 int vfl_fork_token_rows(int32_t* tokens, int64_t row_stride, int32_t num_rows, int32_t width,
                         const int32_t* born, int32_t num_born, void* stream);
+
+/* ---- a decode step in fewer bits ------------------------------------------------------------
+ * (new: no reference counterpart - the reference's caches and weights are 16 or 32 bits wide.)
+ *
+ * The 8-bit paged cache. Codes: int8 [num_blocks, num_kv_heads, block_size, head_dim],
+ * contiguous; scales: float32 [num_blocks, num_kv_heads], contiguous; a cached element is
+ * code * scale. K and V have codes and scales of their own. Blocks that were never written may
+ * hold anything.
+ *
+ * vfl_reshape_and_cache_int8 stores the tokens of key / value (as vfl_reshape_and_cache) at
+ * their slots, in 8 bits. For each run of consecutive tokens in one block, and each head, with a
+ * the largest finite magnitude of the run:
+ *     s' = max(s, a * (1/127)), s = the block's scale, 0 when the run writes offset 0 (the block
+ *          starts anew) or when it is not above 0; a * (1/127) below 2^-100 counts as 0;
+ *     codes the block holds become rint(code * (s * (1/s'))) when s' > s and it did not start anew;
+ *     new codes are rint(x * (1/s')) held to [-127, 127], 0 when s' is 0.
+ * Infinities are held to +-127 and NaNs to 0, flagged VFL_DEVERR_NONFINITE. Tokens of one block
+ * that are not neighbours in the call are stored one run after the other, in no set order.
+ * head_dim a multiple of 16; pointers and token strides 16-byte aligned. */
+int vfl_reshape_and_cache_int8(const void* key, const void* value, void* k_cache, void* v_cache,
+                               float* k_scale, float* v_scale, const int64_t* slot_mapping,
+                               int64_t num_tokens, int num_heads, int head_dim, int block_size,
+                               int64_t num_blocks, int64_t key_token_stride,
+                               int64_t value_token_stride, int dtype, void* stream);
+
+/* Reads tokens back: key / value [num_tokens, num_heads, head_dim], contiguous, of `dtype`:
+ * code * scale at slot_mapping[t], zeros for a negative slot (and, flagged VFL_DEVERR_SLOT, for
+ * one past the pool). */
+int vfl_gather_kv_int8(const void* k_cache, const void* v_cache, const float* k_scale,
+                       const float* v_scale, const int64_t* slot_mapping, void* key, void* value,
+                       int64_t num_tokens, int num_heads, int head_dim, int block_size,
+                       int64_t num_blocks, int dtype, void* stream);
+
+/* Launch plan for vfl_attention_with_kv_cache_int8, from host-side lengths. */
+typedef struct vfl_attention_int8_plan {
+  int64_t magic;           /* VFL_INT8_PLAN_MAGIC once filled                                */
+  int32_t num_reqs;
+  int32_t num_heads;       /* query heads, a multiple of num_kv_heads                        */
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t block_size;
+  int32_t dtype;           /* of query and output                                            */
+  int32_t causal;
+  int32_t total_q;         /* query rows = query_start_loc[num_reqs]                         */
+  int32_t max_q_len;       /* longest request in query rows                                  */
+  int32_t max_seq_len;     /* longest request in cached tokens                               */
+  int32_t tiles_per_split; /* 16-token tiles of one work item                                */
+  int32_t num_splits;      /* work items of the longest request                              */
+  int64_t workspace_bytes; /* scratch the caller must pass (0 = none)                        */
+} vfl_attention_int8_plan;
+
+#define VFL_INT8_PLAN_MAGIC 0x3851504c4656LL /* "VFLPQ8" */
+
+/* As vfl_plan_attention, for the 8-bit cache; num_heads may be a multiple of num_kv_heads. */
+int vfl_plan_attention_int8(int num_reqs, int num_heads, int num_kv_heads, int head_dim,
+                            int block_size, int dtype, int causal, const int32_t* seq_lens_host,
+                            const int32_t* query_start_loc_host, vfl_attention_int8_plan* plan);
+
+/* As vfl_attention_with_kv_cache, over the 8-bit cache. Query head h reads K/V head
+ * h / (num_heads / num_kv_heads). Sums, softmax statistics and the output before its last
+ * rounding are float32. A V scale of 0 says that the block's codes are 0 (as the append leaves
+ * them); V scales below 2^-100 count as 2^-100. */
+int vfl_attention_with_kv_cache_int8(const vfl_attention_int8_plan* plan, const void* query,
+                                     int64_t query_token_stride, const void* k_cache,
+                                     const void* v_cache, const float* k_scale,
+                                     const float* v_scale, int64_t num_blocks, void* output,
+                                     int64_t output_token_stride, const int32_t* query_start_loc,
+                                     const int32_t* seq_lens, const int32_t* block_table,
+                                     int64_t table_stride, int32_t table_cols, float scale,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Linear layer with 4-bit weights: y[m, j] = act(sum_i x[m, i] * scales[j, i / group_size] *
+ * (code(j, i) - 8) + bias[j]) for m < rows, j < n, i < k. codes: uint8 [n, k / 2], element i of a
+ * row in the lower (even i) or upper (odd i) half of byte i / 2; scales: [n, k / group_size], bias
+ * [n] or NULL, x and y of `dtype`; sums in float32. group_size 32, 64 or a multiple of 128, k a
+ * multiple of it; x, its rows and codes 16-byte aligned; strides in elements. Made for a decode
+ * step's few rows (any number is taken). Extends vfl_decode_linear. */
+int vfl_linear_int4(const void* x, int64_t x_stride, const void* codes, const void* scales,
+                    const void* bias, void* y, int64_t y_stride, int32_t rows, int32_t n, int32_t k,
+                    int32_t group_size, int32_t dtype, int32_t activation, void* stream);
+
+/* Scores of given tokens: for row r of `logits` (vocab entries, row_stride elements apart, any
+ * alignment), with p = softmax(row):
+ *     logprobs[r] = ln p[targets[r]] (0 for a negative target; NaN, flagged VFL_DEVERR_SLOT, for
+ *                   one past vocab; targets NULL: none given),
+ *     entropy[r]  = -sum p ln p,
+ *     values / indices [rows, k]: the k largest entries as ln p, value descending, equal values
+ *                   by lower index. k in [0, 64], at most vocab.
+ * Entries of -inf have probability 0. A row of -inf alone has log probabilities of -inf and
+ * entropy 0. A row with a NaN or +inf has NaN scores; NaN entries are no alternatives (index -1
+ * where fewer than k are left). One launch; no workspace. */
+int vfl_token_logprobs(const void* logits, int32_t dtype, int64_t rows, int64_t vocab,
+                       int64_t row_stride, const int32_t* targets, int32_t k, float* logprobs,
+                       float* entropy, float* values, int32_t* indices, void* stream);
 
 #ifdef __cplusplus
 }

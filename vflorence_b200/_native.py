@@ -30,8 +30,10 @@ DEVERR_SLOT = 0x2
 DEVERR_CONTEXT = 0x4
 DEVERR_TIMEOUT = 0x8
 DEVERR_QUERY = 0x10
+DEVERR_NONFINITE = 0x20
 
 PLAN_MAGIC = 0x31504C4656
+INT8_PLAN_MAGIC = 0x3851504C4656
 MAX_COPY_LAYERS = 128
 STATIC_WORKSPACE_BYTES = 64 * 1024 * 1024
 
@@ -63,6 +65,12 @@ EXPORTS = (
     "vfl_row_topk_workspace_size",
     "vfl_beam_merge",
     "vfl_fork_token_rows",
+    "vfl_reshape_and_cache_int8",
+    "vfl_gather_kv_int8",
+    "vfl_plan_attention_int8",
+    "vfl_attention_with_kv_cache_int8",
+    "vfl_linear_int4",
+    "vfl_token_logprobs",
     # host decode runtime (vflorence_b200_runtime.h)
     "vfl_rt_create",
     "vfl_rt_destroy",
@@ -117,6 +125,30 @@ class AttentionPlan(ctypes.Structure):
 PLAN_BYTES = ctypes.sizeof(AttentionPlan)
 
 
+class AttentionInt8Plan(ctypes.Structure):
+    """Mirror of ``vfl_attention_int8_plan``."""
+
+    _fields_ = [
+        ("magic", ctypes.c_int64),
+        ("num_reqs", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("total_q", ctypes.c_int32),
+        ("max_q_len", ctypes.c_int32),
+        ("max_seq_len", ctypes.c_int32),
+        ("tiles_per_split", ctypes.c_int32),
+        ("num_splits", ctypes.c_int32),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+INT8_PLAN_BYTES = ctypes.sizeof(AttentionInt8Plan)
+
+
 class DecodeRules(ctypes.Structure):
     """Mirror of ``vfl_decode_rules``."""
 
@@ -163,6 +195,7 @@ _lib = None
 def _declare(L):
     vp, i32, i64, f32, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
     plan_p = ctypes.POINTER(AttentionPlan)
+    int8_plan_p = ctypes.POINTER(AttentionInt8Plan)
     sig = {
         "vfl_abi_version": (i32, []),
         "vfl_status_string": (ctypes.c_char_p, [i32]),
@@ -193,6 +226,13 @@ def _declare(L):
         "vfl_row_topk_workspace_size": (sz, [i64, i64, i32]),
         "vfl_beam_merge": (i32, [vp, vp, i64, i32, vp, vp, i32, i32, vp, vp]),
         "vfl_fork_token_rows": (i32, [vp, i64, i32, i32, vp, i32, vp]),
+        "vfl_reshape_and_cache_int8": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i64, i64, i64, i32, vp]),
+        "vfl_gather_kv_int8": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i64, i32, vp]),
+        "vfl_plan_attention_int8": (i32, [i32, i32, i32, i32, i32, i32, i32, vp, vp, int8_plan_p]),
+        "vfl_attention_with_kv_cache_int8": (i32, [vp, vp, i64, vp, vp, vp, vp, i64, vp, i64, vp, vp, vp, i64, i32,
+                                                   f32, vp, sz, vp]),
+        "vfl_linear_int4": (i32, [vp, i64, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, vp]),
+        "vfl_token_logprobs": (i32, [vp, i32, i64, i64, i64, vp, i32, vp, vp, vp, vp, vp]),
         "vfl_rt_create": (i32, [i32, i32, i32, i32, ctypes.POINTER(vp)]),
         "vfl_rt_destroy": (None, [vp]),
         "vfl_rt_reset": (i32, [vp]),

@@ -637,3 +637,228 @@ def decode_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
                                    rows, n, k, _dtype_code(x.dtype), _ACTS[activation], _stream(dev))
     N.check(st, "decode_linear")
     return out
+
+
+# ------------------------------------------------------------------------- 8-bit paged cache
+
+def _int8_cache_checks(k_cache, v_cache, k_scale, v_scale):
+    """(device, blocks, heads, block_size, head_dim) of an 8-bit cache: int8 codes
+    [num_blocks, heads, block_size, head_dim] and float32 scales [num_blocks, heads]."""
+    dev = k_cache.device
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k_scale", k_scale), ("v_scale", v_scale)):
+        _require_cuda(name, t, dev)
+    if k_cache.dtype != torch.int8 or v_cache.dtype != torch.int8 or k_cache.dim() != 4 \
+            or v_cache.shape != k_cache.shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("vflorence_b200: 8-bit caches must be contiguous int8 [num_blocks, heads, block_size, head_dim]")
+    n, h, bs, d = k_cache.shape
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32 or k_scale.shape != (n, h) \
+            or v_scale.shape != (n, h) or not (k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise ValueError("vflorence_b200: 8-bit cache scales must be contiguous float32 [num_blocks, heads]")
+    return dev, n, h, bs, d
+
+
+def reshape_and_cache_int8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                           k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """``reshape_and_cache`` into an 8-bit cache: codes int8 [num_blocks, heads, block_size,
+    head_dim] and one float32 scale for each block and head, value = code * scale.
+
+    A block's scale is its largest magnitude / 127. It grows when a larger token arrives (the
+    codes it holds are then rounded to the new step), and starts anew with the block's first slot.
+    Each run of consecutive rows in one block is rounded once, so write a block's tokens as
+    neighbouring rows. Infinities and NaNs are held to +-127 steps and 0, and flagged
+    (``read_device_errors``, DEVERR_NONFINITE)."""
+    dev, n, h, bs, d = _int8_cache_checks(k_cache, v_cache, k_scale, v_scale)
+    _require_cuda("key", key, dev)
+    _require_cuda("value", value, dev)
+    slot_mapping = _on_device("slot_mapping", slot_mapping, dev)
+    _require_dense_rows("key", key)
+    _require_dense_rows("value", value)
+    if key.shape != value.shape or key.dtype != value.dtype or key.shape[1:] != (h, d):
+        raise ValueError(f"vflorence_b200: key and value must be [tokens, {h}, {d}] of one dtype")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1 or slot_mapping.numel() != key.shape[0]:
+        raise ValueError("vflorence_b200: slot_mapping must be int64 [num_tokens]")
+    slots = slot_mapping if slot_mapping.is_contiguous() else slot_mapping.contiguous()
+    st = N.lib().vfl_reshape_and_cache_int8(key.data_ptr(), value.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                            k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr(), key.shape[0], h,
+                                            d, bs, n, key.stride(0), value.stride(0), _dtype_code(key.dtype),
+                                            _stream(dev))
+    N.check(st, "reshape_and_cache_int8")
+
+
+def gather_kv_int8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                   slot_mapping: torch.Tensor, dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """Tokens of an 8-bit cache as (key, value) [tokens, heads, head_dim] of ``dtype`` (code *
+    scale, rounded once); zeros for negative slots. Feeds ``reshape_and_cache`` when a sequence
+    moves to a full-precision cache."""
+    dev, n, h, bs, d = _int8_cache_checks(k_cache, v_cache, k_scale, v_scale)
+    slot_mapping = _on_device("slot_mapping", slot_mapping, dev)
+    if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1:
+        raise ValueError("vflorence_b200: slot_mapping must be int64 [num_tokens]")
+    slots = slot_mapping if slot_mapping.is_contiguous() else slot_mapping.contiguous()
+    code = _dtype_code(dtype)
+    t = slots.numel()
+    key, value = torch.empty((2, t, h, d), dtype=dtype, device=dev).unbind(0)
+    st = N.lib().vfl_gather_kv_int8(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                    slots.data_ptr(), key.data_ptr(), value.data_ptr(), t, h, d, bs, n, code,
+                                    _stream(dev))
+    N.check(st, "gather_kv_int8")
+    return key, value
+
+
+def get_scheduler_metadata_int8(num_reqs: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                                seq_lens: torch.Tensor, dtype: torch.dtype, query_start_loc: torch.Tensor | None,
+                                causal: bool, block_size: int) -> torch.Tensor:
+    """Launch plan for ``attention_with_kv_cache_int8``: a host int64 tensor holding the plan
+    struct. ``dtype`` is the queries'; ``num_heads`` may be a multiple of ``num_kv_heads``."""
+    lens = _host_int32(seq_lens)
+    if lens.numel() != num_reqs:
+        raise ValueError(f"vflorence_b200: seq_lens has {lens.numel()} entries for {num_reqs} requests")
+    qsl = _host_int32(query_start_loc)
+    if qsl is not None and qsl.numel() != num_reqs + 1:
+        raise ValueError("vflorence_b200: query_start_loc must have num_reqs + 1 entries")
+    meta = torch.zeros(N.INT8_PLAN_BYTES // 8, dtype=torch.int64)
+    st = N.lib().vfl_plan_attention_int8(int(num_reqs), int(num_heads), int(num_kv_heads), int(head_dim),
+                                         int(block_size), _dtype_code(dtype), int(bool(causal)),
+                                         lens.data_ptr() if num_reqs else None,
+                                         qsl.data_ptr() if qsl is not None else None,
+                                         N.AttentionInt8Plan.from_address(meta.data_ptr()))
+    N.check(st, "get_scheduler_metadata_int8")
+    return meta
+
+
+def plan_of_int8(metadata: torch.Tensor) -> N.AttentionInt8Plan:
+    """View the plan struct stored in a ``get_scheduler_metadata_int8`` tensor (no copy)."""
+    if (metadata.device.type != "cpu" or metadata.dtype != torch.int64 or not metadata.is_contiguous()
+            or metadata.numel() * 8 < N.INT8_PLAN_BYTES):
+        raise ValueError("vflorence_b200: scheduler_metadata must come from get_scheduler_metadata_int8")
+    plan = N.AttentionInt8Plan.from_buffer(metadata.numpy())
+    if plan.magic != N.INT8_PLAN_MAGIC:
+        raise ValueError("vflorence_b200: scheduler_metadata must come from get_scheduler_metadata_int8")
+    return plan
+
+
+def attention_with_kv_cache_int8(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                 k_scale: torch.Tensor, v_scale: torch.Tensor, output: torch.Tensor,
+                                 query_start_loc: torch.Tensor, seq_lens: torch.Tensor, scale: float, causal: bool,
+                                 block_table: torch.Tensor, scheduler_metadata: torch.Tensor) -> None:
+    """``attention_with_kv_cache`` over an 8-bit cache (``reshape_and_cache_int8``): ``output =
+    softmax(scale * q K^T) V`` per request over its paged tokens. Queries and output are float32
+    or bfloat16; query head h reads K/V head ``h // (num_heads // num_kv_heads)``. Rows that see
+    no token are zeros. ``query_start_loc``, ``seq_lens`` and ``block_table`` may be host tensors."""
+    plan = plan_of_int8(scheduler_metadata)
+    dev, n, h, bs, d = _int8_cache_checks(k_cache, v_cache, k_scale, v_scale)
+    _require_cuda("query", query, dev)
+    _require_cuda("output", output, dev)
+    query_start_loc = _on_device("query_start_loc", query_start_loc, dev)
+    seq_lens = _on_device("seq_lens", seq_lens, dev)
+    block_table = _on_device("block_table", block_table, dev)
+    _require_dense_rows("query", query)
+    _require_dense_rows("output", output)
+    if (plan.num_kv_heads, plan.head_dim, plan.block_size, plan.dtype) != (h, d, bs, _dtype_code(query.dtype)):
+        raise ValueError("vflorence_b200: scheduler_metadata was planned for another cache shape or dtype")
+    if bool(plan.causal) != bool(causal):
+        raise ValueError("vflorence_b200: scheduler_metadata was planned with another causal flag")
+    if output.dtype != query.dtype or query.shape != output.shape or query.shape[1:] != (plan.num_heads, d) \
+            or query.shape[0] < plan.total_q:
+        raise ValueError("vflorence_b200: query/output must be [num_tokens >= planned rows, heads, head_dim] of one dtype")
+    if (query_start_loc.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_table.dtype != torch.int32
+            or block_table.dim() != 2 or block_table.stride(1) != 1 or not seq_lens.is_contiguous()
+            or not query_start_loc.is_contiguous()):
+        raise ValueError("vflorence_b200: query_start_loc, seq_lens and block_table must be int32 "
+                         "(block_table [num_reqs, cols] with unit column stride)")
+    if seq_lens.numel() != plan.num_reqs or query_start_loc.numel() != plan.num_reqs + 1 \
+            or block_table.shape[0] < plan.num_reqs:
+        raise ValueError("vflorence_b200: metadata planned for a different number of requests")
+    ws_bytes = plan.workspace_bytes
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
+    st = N.lib().vfl_attention_with_kv_cache_int8(
+        ctypes.byref(plan), query.data_ptr(), query.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), n, output.data_ptr(), output.stride(0), query_start_loc.data_ptr(),
+        seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], float(scale),
+        ws.data_ptr() if ws is not None else None, ws_bytes, _stream(dev))
+    N.check(st, "attention_with_kv_cache_int8")
+
+
+# ---------------------------------------------------------------------------- 4-bit linear
+
+def quantize_int4(weight: torch.Tensor, group_size: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, scales) of a [n, k] weight for ``linear_int4``: weight[j, i] is about
+    (code - 8) * scales[j, i // group_size], the scale a group's largest magnitude / 7 in the
+    weight's dtype, codes packed two a byte (even i in the lower half): uint8 [n, k // 2]."""
+    if weight.dim() != 2 or weight.dtype not in _DTYPES:
+        raise ValueError("vflorence_b200: quantize_int4 takes a float32 or bfloat16 weight [n, k]")
+    n, k = weight.shape
+    if group_size not in (32, 64) and (group_size <= 0 or group_size % 128) or k % group_size:
+        raise ValueError(f"vflorence_b200: group_size {group_size} must be 32, 64 or a multiple of 128 that divides k = {k}")
+    w = weight.float().view(n, k // group_size, group_size)
+    scales = (w.abs().amax(-1) / 7.0).to(weight.dtype)
+    step = scales.float()[..., None]
+    codes = torch.where(step > 0, w / step, 0.0).round().clamp(-8, 7).add(8).to(torch.uint8).view(n, k // 2, 2)
+    return (codes[..., 0] | (codes[..., 1] << 4)).contiguous(), scales.contiguous()
+
+
+def linear_int4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None,
+                activation: str | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x @ W.T + bias)`` with the 4-bit weight ``quantize_int4`` makes: x [rows, k] float32 or
+    bfloat16 (unit column stride), codes uint8 [n, k // 2], scales [n, k // group_size] and bias [n] of x's
+    dtype; float32 sums, the exact GELU fused. For the few rows of a decode step (any number is
+    taken). Returns ``out`` (a new [rows, n] tensor when None)."""
+    dev = codes.device
+    _require_cuda("codes", codes, dev)
+    _require_cuda("x", x, dev)
+    _require_cuda("scales", scales, dev)
+    if activation not in _ACTS:
+        raise ValueError(f"vflorence_b200: linear_int4 activation {activation!r} (None or 'gelu')")
+    if x.dim() != 2 or codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.uint8 or x.stride(1) != 1 \
+            or x.shape[1] != 2 * codes.shape[1] or not (codes.is_contiguous() and scales.is_contiguous()):
+        raise ValueError("vflorence_b200: linear_int4 takes x [rows, k] (unit column stride), contiguous uint8 codes "
+                         "[n, k / 2] and contiguous scales [n, k / group_size]")
+    rows, k = x.shape
+    n, groups = scales.shape
+    if n != codes.shape[0] or groups == 0 or k % groups:
+        raise ValueError("vflorence_b200: linear_int4 scales must be [n, k / group_size]")
+    if scales.dtype != x.dtype or (bias is not None and (bias.dtype != x.dtype or bias.shape != (n,)
+                                                         or not bias.is_contiguous())):
+        raise ValueError("vflorence_b200: linear_int4 x, scales and bias must share one dtype; bias contiguous [n]")
+    if bias is not None:
+        _require_cuda("bias", bias, dev)
+    if out is None:
+        out = torch.empty((rows, n), dtype=x.dtype, device=dev)
+    elif out.shape != (rows, n) or out.dtype != x.dtype or out.stride(1) != 1 or out.device != dev:
+        raise ValueError("vflorence_b200: linear_int4 out must be [rows, n] of x's dtype with unit column stride")
+    st = N.lib().vfl_linear_int4(x.data_ptr(), x.stride(0) if rows > 1 else k, codes.data_ptr(), scales.data_ptr(),
+                                 bias.data_ptr() if bias is not None else None, out.data_ptr(),
+                                 out.stride(0) if rows > 1 else n, rows, n, k, k // groups, _dtype_code(x.dtype),
+                                 _ACTS[activation], _stream(dev))
+    N.check(st, "linear_int4")
+    return out
+
+
+# -------------------------------------------------------------------------- token scores
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None, k: int = 0):
+    """Scores of given tokens under [rows, vocab] float32/bfloat16 logits (unit column stride, any
+    alignment): (log probability of ``targets`` [rows], entropy [rows], values [rows, k], indices
+    [rows, k]) - all float32 but the int32 indices. ``targets``: int32 [rows]; a negative one
+    scores 0, None scores 0 everywhere. values / indices: each row's ``k`` (at most 64) most
+    likely tokens, log probability descending, ties by lower index. Entries of -inf have
+    probability 0; a row with a NaN or +inf scores NaN."""
+    _require_cuda("logits", logits)
+    dev = logits.device
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("vflorence_b200: token_logprobs wants a [rows, vocab] matrix with unit column stride")
+    rows, vocab = logits.shape
+    if targets is not None:
+        _require_cuda("targets", targets, dev)
+        if targets.dtype != torch.int32 or targets.shape != (rows,) or not targets.is_contiguous():
+            raise ValueError("vflorence_b200: token_logprobs targets must be contiguous int32 [rows]")
+    scores = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    values = torch.empty((rows, k), dtype=torch.float32, device=dev)
+    indices = torch.empty((rows, k), dtype=torch.int32, device=dev)
+    at = scores.data_ptr()
+    st = N.lib().vfl_token_logprobs(logits.data_ptr(), _dtype_code(logits.dtype), rows, vocab,
+                                    logits.stride(0) if rows > 1 else vocab,
+                                    None if targets is None else targets.data_ptr(), int(k), at, at + 4 * rows,
+                                    values.data_ptr() if k else None, indices.data_ptr() if k else None, _stream(dev))
+    N.check(st, "token_logprobs")
+    return scores[0], scores[1], values, indices
