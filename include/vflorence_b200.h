@@ -399,8 +399,9 @@ typedef struct vfl_attention_int8_plan {
   int32_t total_q;         /* query rows = query_start_loc[num_reqs]                         */
   int32_t max_q_len;       /* longest request in query rows                                  */
   int32_t max_seq_len;     /* longest request in cached tokens                               */
-  int32_t tiles_per_split; /* 16-token tiles of one work item                                */
-  int32_t num_splits;      /* work items of the longest request                              */
+  int32_t rows_per_cta;    /* query rows (tokens x heads of a K/V head) a CTA takes: 8 or 16 */
+  int32_t num_splits;      /* CTAs that share a context                                      */
+  int32_t cluster;         /* of them in a thread-block cluster: 1, 2, 4 or 8                */
   int64_t workspace_bytes; /* scratch the caller must pass (0 = none)                        */
 } vfl_attention_int8_plan;
 

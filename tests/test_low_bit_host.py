@@ -45,8 +45,8 @@ def test_plan_splits_few_long_requests_and_covers_them(native):
 
     for lens, kv in (([4096], 16), ([100000], 1), ([1, 2000, 64], 4), ([0, 0], 2), ([15], 3), ([2048] * 512, 16)):
         p = ops.plan_of_int8(_plan(lens, heads=kv, kv=kv))
-        assert p.num_splits * p.tiles_per_split * 16 >= max(lens)
-        assert (p.workspace_bytes == 0) == (p.num_splits == 1)
+        assert p.cluster in (1, 2, 4, 8) and p.num_splits % p.cluster == 0
+        assert (p.workspace_bytes == 0) == (p.num_splits == p.cluster)
     assert ops.plan_of_int8(_plan([100000], heads=1, kv=1)).num_splits > 64
     assert ops.plan_of_int8(_plan([2048] * 512, heads=16, kv=16)).num_splits == 1
     p = ops.plan_of_int8(_plan([], heads=4, kv=4))
@@ -91,7 +91,7 @@ def test_attention_refuses_bad_arguments(native):
                 dict(o_stride=256), dict(t_stride=4), dict(kc=PTR + 1), dict(query=PTR + 8),
                 dict(scale=float("nan")), dict(scale=float("inf"))):
         assert _attend(native, plan, **bad) == 1, bad
-    split_meta = _plan([9000])
+    split_meta = _plan([9000], heads=8, kv=8, d=64)
     split = ops.plan_of_int8(split_meta)
     assert split.workspace_bytes > 0
     assert _attend(native, split, cols=600, t_stride=600) == 3
@@ -101,14 +101,16 @@ def test_attention_refuses_bad_arguments(native):
 
 
 @pytest.mark.parametrize("field,value", [("num_heads", 7), ("num_kv_heads", 0), ("head_dim", 40), ("block_size", 17),
-                                         ("dtype", 5), ("causal", 2), ("num_splits", 0), ("tiles_per_split", 1),
+                                         ("dtype", 5), ("causal", 2), ("num_splits", 0), ("cluster", 3), ("cluster", 0),
+                                         ("num_splits", 12), ("rows_per_cta", 4), ("rows_per_cta", 16),
                                          ("total_q", -1), ("max_q_len", 70000), ("workspace_bytes", 8),
                                          ("num_splits", 70000)])
 def test_attention_refuses_a_corrupted_plan(native, field, value):
     from vflorence_b200 import paged_ops as ops
 
-    meta = _plan([9000, 300])
+    meta = _plan([9000, 300], d=160, heads=1, kv=1)
     plan = ops.plan_of_int8(meta)
+    assert plan.num_splits > plan.cluster == 8
     setattr(plan, field, value)
     assert _attend(native, plan, cols=600, t_stride=600, ws=PTR, ws_bytes=1 << 40) == 1
 

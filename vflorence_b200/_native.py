@@ -140,8 +140,9 @@ class AttentionInt8Plan(ctypes.Structure):
         ("total_q", ctypes.c_int32),
         ("max_q_len", ctypes.c_int32),
         ("max_seq_len", ctypes.c_int32),
-        ("tiles_per_split", ctypes.c_int32),
+        ("rows_per_cta", ctypes.c_int32),
         ("num_splits", ctypes.c_int32),
+        ("cluster", ctypes.c_int32),
         ("workspace_bytes", ctypes.c_int64),
     ]
 
