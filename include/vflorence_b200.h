@@ -402,6 +402,7 @@ typedef struct vfl_attention_int8_plan {
   int32_t rows_per_cta;    /* query rows (tokens x heads of a K/V head) a CTA takes: 8 or 16 */
   int32_t num_splits;      /* CTAs that share a context                                      */
   int32_t cluster;         /* of them in a thread-block cluster: 1, 2, 4 or 8                */
+  int32_t warps;           /* of a CTA, each with tiles of its own: 1, 2, 4 or 8             */
   int64_t workspace_bytes; /* scratch the caller must pass (0 = none)                        */
 } vfl_attention_int8_plan;
 
@@ -411,6 +412,10 @@ typedef struct vfl_attention_int8_plan {
 int vfl_plan_attention_int8(int num_reqs, int num_heads, int num_kv_heads, int head_dim,
                             int block_size, int dtype, int causal, const int32_t* seq_lens_host,
                             const int32_t* query_start_loc_host, vfl_attention_int8_plan* plan);
+
+/* Re-plans `plan` for CTAs of `warps` warps and about num_splits CTAs a context (0: as planned);
+ * updates workspace_bytes. */
+int vfl_plan_attention_int8_shape(vfl_attention_int8_plan* plan, int warps, int num_splits);
 
 /* As vfl_attention_with_kv_cache, over the 8-bit cache. Query head h reads K/V head
  * h / (num_heads / num_kv_heads). Sums, softmax statistics and the output before its last

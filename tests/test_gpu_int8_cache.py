@@ -267,11 +267,22 @@ def attention_exact(q, cache, qsl, lens, table, scale, causal):
     return out, top
 
 
-def attend(q, cache, qsl, lens, table, scale, causal, planned=None, out=None):
+@pytest.fixture(params=[0, 1, 8])
+def warps(request):
+    """Warps a CTA: as planned, and the fewest and most."""
+    return request.param
+
+
+def attend(warps, q, cache, qsl, lens, table, scale, causal, planned=None, out=None):
     dev = [t.cuda() for t in cache]
     meta = ops.get_scheduler_metadata_int8(len(lens), q.shape[1], cache[0].shape[1], q.shape[2],
                                            lens if planned is None else planned, q.dtype, qsl, causal,
                                            cache[0].shape[2])
+    if warps:
+        try:
+            ops.set_shape_int8(meta, warps)
+        except ValueError:
+            pytest.skip("rings of 8 warps do not fit at this head_dim")
     qd = q.cuda()
     out = torch.full_like(qd, 7.0) if out is None else out
     ops.attention_with_kv_cache_int8(qd, *dev, out, qsl.cuda(), lens.cuda(), scale, causal, table.cuda(), meta)
@@ -310,10 +321,10 @@ def batch(lens, rows_per, hkv, group, d, bs, dtype, seed=0, spare=3):
 
 @pytest.mark.parametrize("d", sorted(ops.HEAD_DIMS))
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_attention_head_dims(d, dtype):
+def test_attention_head_dims(warps, d, dtype):
     q, cache, qsl, lens, table = batch([1, 16, 17, 100, 0], [1, 1, 3, 2, 1], 2, 1, d, 16, dtype, seed=d)
     want, top = attention_exact(q, cache, qsl, lens, table, d ** -0.5, False)
-    got, _ = attend(q, cache, qsl, lens, table, d ** -0.5, False)
+    got, _ = attend(warps, q, cache, qsl, lens, table, d ** -0.5, False)
     assert_close(got, want, top, dtype)
     assert (got[int(qsl[4]):] == 0).all()  # a request without tokens
 
@@ -323,28 +334,28 @@ def test_attention_head_dims(d, dtype):
     (1, 1, [9, 17, 1, 3], True), (2, 8, [3, 0, 4, 30], True), (1, 16, [2, 2, 2, 2], True),
 ])
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_attention_grouped_heads_and_causal_rows(hkv, group, rows_per, causal, dtype):
+def test_attention_grouped_heads_and_causal_rows(warps, hkv, group, rows_per, causal, dtype):
     """Requests with more causal rows than tokens hold rows that see nothing."""
     q, cache, qsl, lens, table = batch([3, 33, 64, 21], rows_per, hkv, group, 64, 32, dtype, seed=group)
     want, top = attention_exact(q, cache, qsl, lens, table, 0.2, causal)
-    got, _ = attend(q, cache, qsl, lens, table, 0.2, causal)
+    got, _ = attend(warps, q, cache, qsl, lens, table, 0.2, causal)
     assert_close(got, want, top, dtype)
     assert (got[top == 0] == 0).all()
 
 
 @pytest.mark.parametrize("bs", [16, 48, 64, 1024])
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_attention_block_sizes_and_splits(bs, dtype):
+def test_attention_block_sizes_and_splits(warps, bs, dtype):
     """One long request next to short ones: its context is split and the pieces merged."""
     q, cache, qsl, lens, table = batch([1500, 1, 400, 17], [2, 1, 1, 3], 2, 1, 64, bs, dtype, seed=bs)
     want, top = attention_exact(q, cache, qsl, lens, table, 0.125, False)
-    got, plan = attend(q, cache, qsl, lens, table, 0.125, False)
-    assert plan.num_splits > 1
+    got, plan = attend(warps, q, cache, qsl, lens, table, 0.125, False)
+    assert plan.num_splits > plan.cluster
     assert_close(got, want, top, dtype)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_attention_scales_of_very_different_size(dtype):
+def test_attention_scales_of_very_different_size(warps, dtype):
     """K and V scales that differ by many powers of ten from block to block, and zero scales."""
     q, cache, qsl, lens, table = batch([300, 150], [1, 2], 2, 2, 64, 16, dtype, seed=4)
     g = torch.Generator().manual_seed(8)
@@ -354,12 +365,12 @@ def test_attention_scales_of_very_different_size(dtype):
     cache[3][zero] = 0.0
     cache[1][zero] = 0
     want, top = attention_exact(q, cache, qsl, lens, table, 0.125, False)
-    got, _ = attend(q, cache, qsl, lens, table, 0.125, False)
+    got, _ = attend(warps, q, cache, qsl, lens, table, 0.125, False)
     assert_close(got, want, top, dtype)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_attention_query_sizes_and_non_finite_rows(dtype):
+def test_attention_query_sizes_and_non_finite_rows(warps, dtype):
     """Rows of very large, very small and zero queries, and a NaN or an infinity in one row, which
     stays in that row and head."""
     q, cache, qsl, lens, table = batch([50], [6], 2, 1, 64, 16, dtype, seed=6)
@@ -369,7 +380,7 @@ def test_attention_query_sizes_and_non_finite_rows(dtype):
     q[3, 0, 5] = math.nan
     q[4, 1] = math.inf
     want, top = attention_exact(q[:3], cache, torch.tensor([0, 3]), lens, table, 0.125, False)
-    got, _ = attend(q, cache, qsl, lens, table, 0.125, False)
+    got, _ = attend(warps, q, cache, qsl, lens, table, 0.125, False)
     assert_close(got[1:3], want[1:3], top[1:3], dtype)
     # the huge row attends to one token alone: its score leads by far
     assert_close(got[:1], want[:1], top[:1], dtype)
@@ -377,7 +388,21 @@ def test_attention_query_sizes_and_non_finite_rows(dtype):
     assert got[3, 1].isfinite().all() and got[4, 0].isfinite().all() and got[5].isfinite().all()
 
 
-def test_attention_strides_stream_and_graph():
+def test_attention_splits_of_every_kind():
+    """One to eight CTAs of a cluster, and several clusters with the launch that adds their pieces."""
+    q, cache, qsl, lens, table = batch([1234, 3, 0, 160], [1, 2, 1, 1], 2, 2, 64, 16, BF16, seed=31)
+    want, top = attention_exact(q, cache, qsl, lens, table, 0.125, False)
+    dev = [t.cuda() for t in cache]
+    for splits in (1, 2, 3, 4, 8, 16, 40, 100):
+        meta = ops.get_scheduler_metadata_int8(4, 4, 2, 64, lens, BF16, qsl, False, 16)
+        plan = ops.plan_of_int8(ops.set_shape_int8(meta, 2, splits))
+        assert plan.num_splits <= splits < plan.num_splits * 2
+        out = torch.full_like(q.cuda(), 7.0)
+        ops.attention_with_kv_cache_int8(q.cuda(), *dev, out, qsl.cuda(), lens.cuda(), 0.125, False, table.cuda(), meta)
+        assert_close(out.cpu(), want, top, BF16)
+
+
+def test_attention_strides_stream_and_graph(warps):
     """Queries and outputs as slices of wider buffers, on a side stream, and replayed from a CUDA
     graph with other lengths than were captured (split plan)."""
     q, cache, qsl, lens, table = batch([700, 333], [1, 1], 4, 1, 64, 16, BF16, seed=12)
@@ -390,6 +415,8 @@ def test_attention_strides_stream_and_graph():
     qv = wide_q[:, :256].unflatten(1, (4, 64))
     meta = ops.get_scheduler_metadata_int8(2, 4, 4, 64, lens, BF16, None, False, 16)
     assert ops.plan_of_int8(meta).num_splits > 1
+    if warps:
+        ops.set_shape_int8(meta, warps, 40)
     lens_d, qsl_d, table_d = lens.cuda(), qsl.cuda(), table.cuda()
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -410,16 +437,31 @@ def test_attention_strides_stream_and_graph():
     assert (ov[1] == 0).all()
 
 
-def test_attention_flags_bad_lengths_blocks_and_rows():
+@pytest.mark.parametrize("group,causal", [(1, False), (3, False), (3, True)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_many_requests_of_every_length(warps, group, causal, dtype):
+    """Hundreds of items with empty requests among them."""
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 90, (150,), generator=g).tolist()
+    lens[7], lens[8], lens[100] = 0, 1, 2000
+    rows = torch.randint(0, 4, (150,), generator=g).tolist()
+    q, cache, qsl, lens, table = batch(lens, rows, 2, group, 64, 16, dtype, seed=5)
+    want, top = attention_exact(q, cache, qsl, lens, table, 0.125, causal)
+    got, _ = attend(warps, q, cache, qsl, lens, table, 0.125, causal)
+    assert_close(got, want, top, dtype)
+    assert (got[top == 0] == 0).all()
+
+
+def test_attention_flags_bad_lengths_blocks_and_rows(warps):
     q, cache, qsl, lens, table = batch([40, 20], [1, 1], 2, 1, 64, 16, BF16, seed=13)
     ops.read_device_errors()
     longer = torch.tensor([49, 20], dtype=torch.int32)  # more than its table holds
-    attend(q, cache, qsl, longer, table, 0.125, False, planned=longer)
+    attend(warps, q, cache, qsl, longer, table, 0.125, False, planned=longer)
     assert ops.read_device_errors() == N.DEVERR_CONTEXT
     broken = table.clone()
     broken[1, 0] = 10 ** 6
     want, top = attention_exact(q[:1], cache, qsl[:2], lens[:1], table, 0.125, False)
-    got, _ = attend(q, cache, qsl, lens, broken, 0.125, False)
+    got, _ = attend(warps, q, cache, qsl, lens, broken, 0.125, False)
     assert ops.read_device_errors() == N.DEVERR_BLOCK_ID
     assert_close(got[:1], want, top, BF16)
     dev = [t.cuda() for t in cache]

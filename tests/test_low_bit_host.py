@@ -104,7 +104,7 @@ def test_attention_refuses_bad_arguments(native):
                                          ("dtype", 5), ("causal", 2), ("num_splits", 0), ("cluster", 3), ("cluster", 0),
                                          ("num_splits", 12), ("rows_per_cta", 4), ("rows_per_cta", 16),
                                          ("total_q", -1), ("max_q_len", 70000), ("workspace_bytes", 8),
-                                         ("num_splits", 70000)])
+                                         ("num_splits", 70000), ("warps", 3), ("warps", 0)])
 def test_attention_refuses_a_corrupted_plan(native, field, value):
     from vflorence_b200 import paged_ops as ops
 

@@ -68,6 +68,7 @@ EXPORTS = (
     "vfl_reshape_and_cache_int8",
     "vfl_gather_kv_int8",
     "vfl_plan_attention_int8",
+    "vfl_plan_attention_int8_shape",
     "vfl_attention_with_kv_cache_int8",
     "vfl_linear_int4",
     "vfl_token_logprobs",
@@ -143,6 +144,7 @@ class AttentionInt8Plan(ctypes.Structure):
         ("rows_per_cta", ctypes.c_int32),
         ("num_splits", ctypes.c_int32),
         ("cluster", ctypes.c_int32),
+        ("warps", ctypes.c_int32),
         ("workspace_bytes", ctypes.c_int64),
     ]
 
@@ -230,6 +232,7 @@ def _declare(L):
         "vfl_reshape_and_cache_int8": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i64, i64, i64, i32, vp]),
         "vfl_gather_kv_int8": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i64, i32, vp]),
         "vfl_plan_attention_int8": (i32, [i32, i32, i32, i32, i32, i32, i32, vp, vp, int8_plan_p]),
+        "vfl_plan_attention_int8_shape": (i32, [int8_plan_p, i32, i32]),
         "vfl_attention_with_kv_cache_int8": (i32, [vp, vp, i64, vp, vp, vp, vp, i64, vp, i64, vp, vp, vp, i64, i32,
                                                    f32, vp, sz, vp]),
         "vfl_linear_int4": (i32, [vp, i64, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, i32, vp]),

@@ -9,19 +9,20 @@
 // out = sum w_t vc_t / sum (w_t / vs_b). Both sums and M are float32; w is at most 2^8 and is
 // rounded to half precision for its product alone (float32 queries: to a pair of halves).
 //
-// The codes are exact in half precision, so both products run on m16n8k16 half-precision tensor
-// instructions with float32 sums. A query row is scaled by a power of two into [-1, 1] (its
-// exponent returns with ks_b); bfloat16 queries are then exact halves down to 2^-14 of the row's
-// largest, float32 ones are split into two halves.
+// Scores: K's codes enter m16n8k32 integer instructions as they are. A query row is brought to
+// whole numbers of 2^-14 (bfloat16) or 2^-22 (float32) of a power of two above its largest
+// element, held as 2 or 3 planes of 8 bits: bfloat16 elements down to 2^-7 of the row's largest
+// are exact, what is smaller is rounded to 2^-15 of it, next to the output's 2^-9. The sums are
+// exact integers. Outputs: V's codes are exact in half precision and meet w in m16n8k16 half
+// instructions with float32 sums.
 //
-// Bound: HBM, 2 D bytes a token and K/V head. What the layout buys: the fragments' index maps are
-// free to choose, because q . kc sums over dims in any order and the softmax over tokens in any
-// order. Scores are taken as K q^T (16 tokens x 8 query rows) and outputs as V^T w^T (16 dims x 8
-// rows), so that the cached elements fill the instruction's 16-row side and a few query rows its
-// 8-column side. A lane's 16 dims of K are 16 neighbouring bytes, its V values 8 neighbouring
-// bytes of four tokens; two 8 x 8 transpositions in registers turn scores into weights. Per tile
-// of 16 tokens and D = 64 that is about 90 integer and half operations a lane to make halves of
-// the codes, 8 tensor instructions, and 25 for the softmax.
+// Bound: HBM, 2 D bytes a token and K/V head, and close behind it the integer pipe that turns V's
+// codes into halves. What the layout buys: scores are taken as K q^T (16 tokens x 8 query rows)
+// and outputs as V^T w^T (16 dims x 8 rows), so that the cached elements fill the instructions'
+// 16-row side and a few query rows their 8-column side. The index maps are free to choose,
+// because q . kc sums over dims in any order and the softmax over tokens in any order: a lane's
+// K operands are 16 neighbouring bytes of two tokens, its V operands come transposed out of a
+// byte matrix load, and two 8 x 8 transpositions in registers turn scores into weights.
 //
 // One CTA takes a request, a K/V head, 8 or 16 query rows (those of the heads that share the K/V
 // head, of all the request's query tokens) and a range of 16-token tiles. Each warp streams its
@@ -41,8 +42,7 @@ namespace cg = cooperative_groups;
 namespace vfl {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
+constexpr int kMaxWarps = 8;
 constexpr int kMaxCluster = 8;
 constexpr int kSmemPerSM = 227 * 1024;
 constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: smaller V scales count as it
@@ -100,20 +100,16 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Where the 32-byte unit `u` of row `row` of a 16 x D byte tile lies: the units of a 128-byte
-// line are permuted so that the eight rows (K) and four rows (V) that a warp reads together
-// fall into different banks.
+// Where byte `byte` of row `row` of a 16 x D byte tile lies: the 16-byte chunks of a 128-byte line
+// are permuted so that the rows that one phase of a warp's loads reads (pairs of K rows 2 apart,
+// eight neighbouring V rows) fall into different banks.
 template <int D>
 __device__ __forceinline__ int tile_offset(int row, int byte) {
-  if (D == 64) {
-    const int line = row >> 1, in_line = (row & 1) * 64 + byte;
-    return line * 128 + (in_line ^ ((line & 3) << 5));
-  }
-  if (D % 128 == 0) {
-    const int x = (row & 3) ^ ((row >> 1) & 2);
-    return row * D + (byte ^ (x << 5));
-  }
-  return row * D + byte;
+  int x = 0;
+  if (D % 128 == 0) x = ((row & 2) << 1) | ((row & 4) >> 1) | (row & 1);
+  if (D == 64) x = ((row >> 1) & 3) | ((row & 2) << 1);
+  if (D == 32) x = (row >> 2) & 1;
+  return (row * D + byte) ^ (x << 4);
 }
 
 // Bytes 0, 2 (shift 0) or 1, 3 (shift 8) of `w`, signed, as two halves: 0x6400 | (b ^ 0x80) is
@@ -137,6 +133,32 @@ __device__ __forceinline__ void mma_half(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Whole numbers: A 16 x 32 (or 16 x 16) of K codes, B of 8-bit query digits.
+__device__ __forceinline__ void mma_int_k32(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_int_k16(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+               : "r"(a0), "r"(a1), "r"(b0));
+}
+
+// 16 x 16 byte matrices whose rows the lanes 0-15 (16-31) address, transposed: lane 4g + tq gets
+// rows 4 tq .. 4 tq + 3 of column g in r[0] (r[2]) and of column g + 8 in r[1] (r[3]).
+__device__ __forceinline__ void load_bytes_trans_x2(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void load_bytes_trans_x1(uint32_t addr, uint32_t& r0, uint32_t& r1) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x1.trans.shared.b8 {%0,%1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(addr) : "memory");
+}
+
 // The 8 x 8 half matrix whose row g the four lanes of group g hold, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
@@ -148,20 +170,20 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 template <typename T, int D, int NT>
 struct Shape {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;  // halves that make up a query element
-  static constexpr int kSteps = D / 16;                  // k16 steps of K q^T
-  static constexpr int kTiles = D / 16;                  // m16 tiles of the output
+  static constexpr int kPlanes = sizeof(T) == 4 ? 3 : 2;  // 8-bit digits of a query element
+  static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;   // halves that make up a weight
+  static constexpr int kWords = D / 16;                   // 4-dim words a lane holds of a row
+  static constexpr int kTiles = D / 16;                   // m16 tiles of the output
   static constexpr int kStageBytes = 2 * 16 * D;
-  static constexpr int kStages = D <= 128 ? 4 : (D <= 256 ? 3 : 2);
+  static constexpr int kStages = D <= 128 ? 4 : 2;
   static constexpr int kRingBytes = kStages * kStageBytes;
-  // query fragments stay in registers up to this many, in shared memory past it
-  static constexpr bool kQueryInSmem = kTerms * NT * kSteps * 2 > 32;
-  static constexpr int kQueryBytes = kQueryInSmem ? kTerms * NT * kSteps * 32 * 8 : 0;
-  static constexpr int kMetaBytes = kWarps * 64 * 16;
-  // sums of the warps [warp][row][D], of the CTA [row][D], and their (m, l)
-  static constexpr int kMergeBytes = ((kWarps + 1) * kRows * (D + 2)) * 4;
-  static constexpr int kRegion = kWarps * kRingBytes > kMergeBytes ? kWarps * kRingBytes : kMergeBytes;
-  static constexpr int kSmem = kRegion + kMetaBytes + kQueryBytes;
+  // query digits stay in registers up to this many, in shared memory past it
+  static constexpr bool kQueryInSmem = kPlanes * NT * kWords > 32;
+  // the warps' rings, later their sums [warp][row][D], the CTA's [row][D] and all their (m, l)
+  __device__ __forceinline__ static int region(int warps) {
+    const int merge = (warps + 1) * kRows * (D + 2) * 4;
+    return warps * kRingBytes > merge ? warps * kRingBytes : merge;
+  }
 };
 
 template <typename T>
@@ -189,47 +211,291 @@ __device__ __forceinline__ float merge_factor(float m, float m_all) {
   return m == -INFINITY ? 1.f : exp2_approx(m - m_all);
 }
 
-// First dim of the word (4 codes) of k16 step s that lane group thread tq holds: whole groups of
-// 64 dims give a thread 16 neighbouring bytes, the rest 4.
+// First dim of word `w` (4 dims) of a row that lane group thread tq holds: whole groups of 64 dims
+// give a thread 16 neighbouring bytes, a group of 32 gives 8, one of 16 gives 4.
 template <int D>
-__device__ __forceinline__ int k_dim(int s, int tq) {
-  constexpr int kWhole = D / 64 * 4;
-  return s < kWhole ? (s >> 2) * 64 + tq * 16 + (s & 3) * 4 : kWhole * 16 + (s - kWhole) * 16 + tq * 4;
+__device__ __forceinline__ int k_dim(int w, int tq) {
+  constexpr int k64 = D / 64, k32 = (D % 64) / 32;
+  if (w < 4 * k64) return (w >> 2) * 64 + tq * 16 + (w & 3) * 4;
+  if (w < 4 * k64 + 2 * k32) return k64 * 64 + tq * 8 + (w - 4 * k64) * 4;
+  return k64 * 64 + k32 * 32 + tq * 4;
 }
 
-// The V dims of a lane: column n of [0, D / 8) is dim start + span * g + (n - start / 8), where
-// spans of 16, 8, 4 and 2 neighbouring dims cover groups of 128, 64, 32 and 16.
-template <int D>
-__device__ __forceinline__ int v_dim(int n, int g) {
-  constexpr int k16 = D / 128, k8 = (D % 128) / 64, k4 = (D % 64) / 32;
-  const int start = n < k16 * 16 ? n / 16 * 128
-                    : n < k16 * 16 + k8 * 8 ? k16 * 128
-                    : n < k16 * 16 + k8 * 8 + k4 * 4 ? k16 * 128 + k8 * 64
-                                                     : k16 * 128 + k8 * 64 + k4 * 32;
-  const int span = n < k16 * 16 ? 16 : n < k16 * 16 + k8 * 8 ? 8 : n < k16 * 16 + k8 * 8 + k4 * 4 ? 4 : 2;
-  return start + span * g + (n - start / 8);
-}
+// A lane's place in the fragments.
+struct Lane {
+  int lane, g, tq, krow;  // krow: token of score row g; row g + 8 holds token krow + 1
+  __device__ __forceinline__ Lane() : lane(threadIdx.x & 31), g(lane >> 2), tq(lane & 3), krow(2 * g) {}
+};
 
-// One query row's four dims of k16 step s as the two B registers of each term.
-template <int kTerms>
-__device__ __forceinline__ void query_halves(float (&f)[4], float inv, uint32_t (&b)[kTerms][2]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] *= inv;
-#pragma unroll
-  for (int term = 0; term < kTerms; ++term) {
-    b[term][0] = pack_half2(f[0], f[2]);
-    b[term][1] = pack_half2(f[1], f[3]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] -= __half2float(__float2half_rn(f[i]));
+// What a lane knows of the query rows: their digits (or where in shared memory they are), the
+// factor of their scores, the tokens they see.
+template <typename T, int D, int NT>
+struct Query {
+  using S = Shape<T, D, NT>;
+  uint32_t digits[S::kQueryInSmem ? 1 : NT * S::kPlanes * S::kWords];
+  const uint32_t* smem;
+  float mul[NT][2];  // of the rows 2 tq, 2 tq + 1 whose scores this lane holds
+  int vis[NT][2];
+  int vis_all;       // tokens that every row sees
+
+  // word `w` of row g of n8 tile nt, plane `plane` (0: the highest digits)
+  __device__ __forceinline__ uint32_t word(int nt, int plane, int w, int lane) const {
+    const int at = (nt * S::kPlanes + plane) * S::kWords + w;
+    return S::kQueryInSmem ? smem[at * 32 + lane] : digits[S::kQueryInSmem ? 0 : at];
   }
-}
+
+  // Rows row0 .. row0 + nrows of a request's rows of one K/V head. `visible(i)`: tokens that row i
+  // of these sees. Warp `warp` stores its share of the digits where they go to shared memory (the
+  // caller syncs).
+  template <typename V>
+  __device__ __forceinline__ void load(const Int8AttnParams& p, const Lane& ln, int warp, int warps, int q_begin, int kvh,
+                                       int group, int row0, int nrows, const V& visible, uint32_t* q_smem) {
+    smem = q_smem;
+    vis_all = visible(0);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = nt * 8 + ln.g;
+      const bool on = row < nrows;
+      const int vrow = row0 + (on ? row : 0);
+      const int token = vrow / group, head = kvh * group + vrow - token * group;
+      const T* src = static_cast<const T*>(p.q) + (int64_t)(q_begin + token) * p.q_stride + (int64_t)head * D;
+      constexpr int kHeld = S::kWords <= 8 ? S::kWords : 1;  // long rows are read twice
+      float f[kHeld][4];
+      float amax = 0.f;
+      bool odd = false;  // an infinity or a NaN
+      auto look = [&](const float (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          amax = fmaxf(amax, fabsf(v[i]));
+          odd |= !(fabsf(v[i]) <= FLT_MAX);
+        }
+      };
+#pragma unroll
+      for (int w = 0; w < S::kWords; ++w) {
+        float(&v)[4] = f[w < kHeld ? w : 0];
+        v[0] = v[1] = v[2] = v[3] = 0.f;
+        if (on) load4(src + k_dim<D>(w, ln.tq), v);
+        if (kHeld == 1) look(v);
+      }
+      if (kHeld > 1) {
+#pragma unroll
+        for (int w = 0; w < kHeld; ++w) look(f[w]);
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const bool bad = ((__ballot_sync(0xffffffffu, odd) >> (ln.lane & ~3)) & 15u) != 0;  // in this lane's row
+      // 2^e > amax >= 2^(e-1), from the exponent bits
+      const int e = max(-90, static_cast<int>(__float_as_uint(amax) >> 23) - 126);
+      constexpr int kBits = S::kPlanes == 3 ? 22 : 14;
+      const float to_int = ldexpf(1.f, kBits - e);
+#pragma unroll
+      for (int w = 0; w < S::kWords; ++w) {
+        float(&v)[4] = f[w < kHeld ? w : 0];
+        if (kHeld == 1) {
+          v[0] = v[1] = v[2] = v[3] = 0.f;
+          if (on) load4(src + k_dim<D>(w, ln.tq), v);
+        }
+        int c[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = __float2int_rn(v[i] * to_int);
+#pragma unroll
+        for (int plane = S::kPlanes - 1; plane >= 0; --plane) {
+          // digits base 256 in [-128, 127], the lowest first
+          uint32_t packed = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            packed |= (uint32_t)(c[i] & 255) << (8 * i);
+            c[i] = (c[i] - (int)(int8_t)c[i]) >> 8;
+          }
+          const int at = (nt * S::kPlanes + plane) * S::kWords + w;
+          if (S::kQueryInSmem) {
+            if (w % warps == warp) q_smem[at * 32 + ln.lane] = packed;
+          } else {
+            digits[S::kQueryInSmem ? 0 : at] = packed;
+          }
+        }
+      }
+      // a row with an infinity or a NaN scores NaN
+      const float row_mul = bad ? NAN : ldexpf(p.scale_log2, e - kBits);
+#pragma unroll
+      for (int e2 = 0; e2 < 2; ++e2) {
+        mul[nt][e2] = __shfl_sync(0xffffffffu, row_mul, (2 * ln.tq + e2) * 4);
+        // columns without a row have scores of zero; as rows that see everything they stay on
+        // the common path
+        const int row2 = nt * 8 + 2 * ln.tq + e2;
+        vis[nt][e2] = row2 < nrows ? visible(row2) : INT32_MAX;
+      }
+    }
+  }
+};
+
+// Running sums of a warp: maximum and sum of the rows 2 tq, 2 tq + 1 and out^T.
+template <typename T, int D, int NT>
+struct Sums {
+  using S = Shape<T, D, NT>;
+  float m[NT][2], l[NT][2];
+  float acc[NT][S::kTiles][4];
+
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[nt][t][e] = 0.f;
+    }
+  }
+
+  // l over the lanes that share a row
+  __device__ __forceinline__ void reduce() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], o);
+  }
+
+  // One 16-token tile in shared memory: K codes at kt, V codes at vt (a shared address); mt = (ks,
+  // log2 vs, 1 / vs); tok0: the tile's first position.
+  __device__ __forceinline__ void tile(const uint8_t* kt, uint32_t vt, const float4& mt, int tok0,
+                                       const Query<T, D, NT>& q, const Lane& ln) {
+    const int tq = ln.tq, krow = ln.krow;
+    // ---- scores: c[0..1] token krow of rows 2 tq, 2 tq + 1; c[2..3] token krow + 1
+    int si[NT][S::kPlanes][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int pl = 0; pl < S::kPlanes; ++pl)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) si[nt][pl][e] = 0;
+    constexpr int k64 = D / 64, k32 = (D % 64) / 32, k16 = (D % 32) / 16;
+    auto pair = [&](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, int w) {  // words w, w + 1
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int pl = 0; pl < S::kPlanes; ++pl)
+          mma_int_k32(si[nt][pl], a0, a1, a2, a3, q.word(nt, pl, w, ln.lane), q.word(nt, pl, w + 1, ln.lane));
+    };
+#pragma unroll
+    for (int c = 0; c < k64; ++c) {
+      const uint4 a = *reinterpret_cast<const uint4*>(kt + tile_offset<D>(krow, c * 64 + tq * 16));
+      const uint4 b = *reinterpret_cast<const uint4*>(kt + tile_offset<D>(krow + 1, c * 64 + tq * 16));
+      pair(a.x, b.x, a.y, b.y, 4 * c);
+      pair(a.z, b.z, a.w, b.w, 4 * c + 2);
+    }
+    if (k32) {
+      const uint2 a = *reinterpret_cast<const uint2*>(kt + tile_offset<D>(krow, k64 * 64 + tq * 8));
+      const uint2 b = *reinterpret_cast<const uint2*>(kt + tile_offset<D>(krow + 1, k64 * 64 + tq * 8));
+      pair(a.x, b.x, a.y, b.y, 4 * k64);
+    }
+    if (k16) {
+      const uint32_t a = *reinterpret_cast<const uint32_t*>(kt + tile_offset<D>(krow, k64 * 64 + k32 * 32 + tq * 4));
+      const uint32_t b = *reinterpret_cast<const uint32_t*>(kt + tile_offset<D>(krow + 1, k64 * 64 + k32 * 32 + tq * 4));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int pl = 0; pl < S::kPlanes; ++pl)
+          mma_int_k16(si[nt][pl], a, b, q.word(nt, pl, 4 * k64 + 2 * k32, ln.lane));
+    }
+    // digits to scores: the two highest planes fit an integer (2^14 * 127 * 512 < 2^31)
+    float sc[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sc[nt][e] = (float)(si[nt][0][e] * 256 + si[nt][1][e]);
+        if (S::kPlanes == 3) sc[nt][e] = fmaf(sc[nt][e], 256.f, (float)si[nt][S::kPlanes - 1][e]);
+      }
+
+    // ---- weights
+    const bool partial = tok0 + 16 > q.vis_all;
+    uint32_t pb[NT][S::kTerms][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float mul[2] = {mt.x * q.mul[nt][0], mt.x * q.mul[nt][1]};
+      float x[4];  // base-2 exponents against the running maximum
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = fmaf(sc[nt][e], mul[e & 1], mt.y - m[nt][e & 1]);
+      if (partial) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (tok0 + krow + (e >> 1) >= q.vis[nt][e & 1]) x[e] = -INFINITY;
+      }
+      // NaN - as for a row that has no maximum yet - compares false: such rows come here too
+      const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      if (__any_sync(0xffffffffu, !(top <= kRescaleSlack))) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float y0 = tok0 + krow < q.vis[nt][e] ? fmaf(sc[nt][e], mul[e], mt.y) : -INFINITY;
+          const float y1 = tok0 + krow + 1 < q.vis[nt][e] ? fmaf(sc[nt][e + 2], mul[e], mt.y) : -INFINITY;
+          float mx = fmaxf(y0, y1);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          float& mr = m[nt][e];
+          if (mx > mr + kRescaleSlack) {
+            const float alpha = mr == -INFINITY ? 0.f : exp2_approx(mr - mx);
+            mr = mx;
+            l[nt][e] *= alpha;
+#pragma unroll
+            for (int t = 0; t < S::kTiles; ++t) {
+              acc[nt][t][e] *= alpha;
+              acc[nt][t][e + 2] *= alpha;
+            }
+          }
+          // a row that has seen no token yet has m = -inf, and -inf - m would be a NaN
+          x[e] = y0 == -INFINITY ? -INFINITY : y0 - mr;
+          x[e + 2] = y1 == -INFINITY ? -INFINITY : y1 - mr;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = exp2_approx(x[e]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) l[nt][e] = fmaf(x[e] + x[e + 2], mt.z, l[nt][e]);
+#pragma unroll
+      for (int term = 0; term < S::kTerms; ++term) {
+        pb[nt][term][0] = transpose8(pack_half2(x[0], x[1]));
+        pb[nt][term][1] = transpose8(pack_half2(x[2], x[3]));
+        if (term + 1 < S::kTerms) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] -= __half2float(__float2half_rn(x[e]));
+        }
+      }
+    }
+
+    // ---- out^T += V^T w^T. A lane's word holds tokens 4 tq .. 4 tq + 3 of a dim: bytes 0 and 2 are
+    // the tokens of score rows 2 tq, 2 tq + 1, bytes 1 and 3 those of rows 2 tq + 8, 2 tq + 9
+    auto product = [&](uint32_t lo, uint32_t hi, int t) {  // dims g and g + 8 of m16 tile t
+      const uint32_t a[4] = {codes_to_half2(lo), codes_to_half2(hi), codes_to_half2(lo >> 8), codes_to_half2(hi >> 8)};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int term = 0; term < S::kTerms; ++term) mma_half(acc[nt][t], a, pb[nt][term][0], pb[nt][term][1]);
+    };
+#pragma unroll
+    for (int t = 0; t + 1 < S::kTiles; t += 2) {  // lanes 0-15 address the rows of tile t, 16-31 of t + 1
+      uint32_t r[4];
+      load_bytes_trans_x2(vt + tile_offset<D>(ln.lane & 15, t * 16 + (ln.lane & 16)), r);
+      product(r[0], r[1], t);
+      product(r[2], r[3], t + 1);
+    }
+    if (S::kTiles % 2) {
+      uint32_t r0, r1;
+      load_bytes_trans_x1(vt + tile_offset<D>(ln.lane & 15, (S::kTiles - 1) * 16), r0, r1);
+      product(r0, r1, S::kTiles - 1);
+    }
+  }
+};
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) paged_attention_int8_kernel(const Int8AttnParams p) {
+__global__ void __launch_bounds__(kMaxWarps * 32) paged_attention_int8_kernel(const Int8AttnParams p) {
   using S = Shape<T, D, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, tq = lane & 3;
+  const Lane ln;
+  const int warp = threadIdx.x >> 5, lane = ln.lane, warps = blockDim.x >> 5;
+  const int region = S::region(warps);
   const int r = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x - r * p.num_kv_heads;
   const int split = blockIdx.z;
   const int bs = p.block_size, tpb = bs >> 4;
@@ -254,13 +520,13 @@ __global__ void __launch_bounds__(kThreads) paged_attention_int8_kernel(const In
   const int tile_begin = split * per;
   const int tile_end = min(tile_begin + per, ceil_div(visible(nrows - 1), 16));
 
-  // ---- this warp's tiles: tile_begin + warp + kWarps * i. A lane keeps the position of one of
+  // ---- this warp's tiles: tile_begin + warp + warps * i. A lane keeps the position of one of
   // 32 tiles in units of 16 tokens of the pools, and of the next 32.
   const int first = tile_begin + warp;
-  const int count = tile_end > first ? ceil_div(tile_end - first, kWarps) : 0;
+  const int count = tile_end > first ? ceil_div(tile_end - first, warps) : 0;
   auto locate = [&](int i) {
     if (i >= count) return 0;
-    const int tile = first + kWarps * i;
+    const int tile = first + warps * i;
     const int col = tpb == 1 ? tile : tile / tpb;
     int b = __ldg(p.table + (int64_t)r * p.table_stride + col);
     if (b < 0 || b >= p.num_blocks) {
@@ -274,6 +540,8 @@ __global__ void __launch_bounds__(kThreads) paged_attention_int8_kernel(const In
   const uint32_t ring_u32 = smem_u32(ring);
   // where this lane's 16-byte pieces of a tile go, within a stage
   constexpr int kPieces = (D + 31) / 32;
+  const int8_t* k_lane = p.k_cache + lane * 16;
+  const int8_t* v_lane = p.v_cache + lane * 16;
   uint32_t piece_at[kPieces];
 #pragma unroll
   for (int j = 0; j < kPieces; ++j) {
@@ -284,13 +552,14 @@ __global__ void __launch_bounds__(kThreads) paged_attention_int8_kernel(const In
   auto issue = [&](int i, int stage) {  // copies tile i into `stage` (a group of its own, empty past the end)
     if (i < count) {
       const int at = __shfl_sync(0xffffffffu, i < base + 32 ? place : place_next, i & 31);
-      const int64_t src = (int64_t)at * (16 * D) + lane * 16;
+      const int8_t* ks = k_lane + (int64_t)at * (16 * D);
+      const int8_t* vs = v_lane + (int64_t)at * (16 * D);
       const uint32_t to = stage * S::kStageBytes;
 #pragma unroll
       for (int j = 0; j < kPieces; ++j) {
         if (D % 32 == 0 || j * 32 + lane < D) {
-          cp_async16(piece_at[j] + to, p.k_cache + src + j * 512);
-          cp_async16(piece_at[j] + to + 16 * D, p.v_cache + src + j * 512);
+          cp_async16(piece_at[j] + to, ks + j * 512);
+          cp_async16(piece_at[j] + to + 16 * D, vs + j * 512);
         }
       }
     }
@@ -300,7 +569,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_int8_kernel(const In
   for (int i = 0; i < S::kStages - 1; ++i) issue(i, i);
 
   // ---- the tiles' scales: (ks, log2 vs, 1 / vs), 64 tiles of them in shared memory
-  float4* meta = reinterpret_cast<float4*>(smem + S::kRegion) + warp * 64;
+  float4* meta = reinterpret_cast<float4*>(smem + region) + warp * 64;
   float ks_next = 0.f, vs_next = 1.f;
   auto load_scales = [&](int i, int at) {
     if (i < count) {
@@ -315,270 +584,61 @@ __global__ void __launch_bounds__(kThreads) paged_attention_int8_kernel(const In
   };
   load_scales(lane, place);
 
-  // ---- the query rows, scaled into [-1, 1], as the B fragments of K q^T
-  uint2* q_smem = reinterpret_cast<uint2*>(smem + S::kRegion + S::kMetaBytes);
-  uint32_t qb[S::kQueryInSmem ? 1 : NT][S::kQueryInSmem ? 1 : S::kSteps][S::kTerms][2];
-  float s_mul[NT][2];  // of the rows 2 tq, 2 tq + 1 whose scores this lane holds
-  int vis[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int row = nt * 8 + g;
-    const bool on = row < nrows;
-    const int vrow = row0 + (on ? row : 0);
-    const int token = vrow / group, head = kvh * group + vrow - token * group;
-    const T* src = static_cast<const T*>(p.q) + (int64_t)(req.q_begin + token) * p.q_stride + (int64_t)head * D;
-    float amax = 0.f;
-#pragma unroll
-    for (int s = 0; s < S::kSteps; ++s) {
-      float f[4] = {0.f, 0.f, 0.f, 0.f};
-      if (on) load4(src + k_dim<D>(s, tq), f);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(f[i]));
-    }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // 2^e > amax >= 2^(e-1); an infinity stays one in the products, as it would unscaled
-    int e = 0;
-    if (amax > 0.f && amax <= FLT_MAX) frexpf(amax, &e);
-    e = max(-125, min(126, e));
-    const float inv = ldexpf(1.f, -e);
-#pragma unroll
-    for (int s = 0; s < S::kSteps; ++s) {
-      float f[4] = {0.f, 0.f, 0.f, 0.f};
-      if (on) load4(src + k_dim<D>(s, tq), f);
-      uint32_t b[S::kTerms][2];
-      query_halves<S::kTerms>(f, inv, b);
-#pragma unroll
-      for (int term = 0; term < S::kTerms; ++term) {
-        if (S::kQueryInSmem) {
-          if (s % kWarps == warp)
-            q_smem[((term * NT + nt) * S::kSteps + s) * 32 + lane] = make_uint2(b[term][0], b[term][1]);
-        } else {
-          qb[S::kQueryInSmem ? 0 : nt][S::kQueryInSmem ? 0 : s][term][0] = b[term][0];
-          qb[S::kQueryInSmem ? 0 : nt][S::kQueryInSmem ? 0 : s][term][1] = b[term][1];
-        }
-      }
-    }
-    const float mul = ldexpf(1.f, e) * p.scale_log2;
-#pragma unroll
-    for (int e2 = 0; e2 < 2; ++e2) {
-      s_mul[nt][e2] = __shfl_sync(0xffffffffu, mul, (2 * tq + e2) * 4);
-      // columns without a row have scores of zero; as rows that see everything they stay on the
-      // common path
-      const int row2 = nt * 8 + 2 * tq + e2;
-      vis[nt][e2] = row2 < nrows ? visible(row2) : INT32_MAX;
-    }
-  }
-  const int vis_all = visible(0);  // tokens that every row sees
+  // ---- the query rows
+  Query<T, D, NT> query;
+  query.load(p, ln, warp, warps, req.q_begin, kvh, group, row0, nrows, visible,
+             reinterpret_cast<uint32_t*>(smem + region + warps * 64 * 16));
   keep_scales(lane);
   if (S::kQueryInSmem) __syncthreads();
+  Sums<T, D, NT> sum;
+  sum.reset();
 
-  float m_run[NT][2], l_run[NT][2];
-  float acc[NT][S::kTiles][4];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m_run[nt][0] = m_run[nt][1] = -INFINITY;
-    l_run[nt][0] = l_run[nt][1] = 0.f;
-#pragma unroll
-    for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[nt][t][e] = 0.f;
-  }
-  const int krow = (g >> 1) + 4 * (g & 1);  // token of score row g; row g + 8 holds token krow + 8
-
-  int stage = 0;
+  // batches of 32 tiles (their places and scales come one batch ahead), in them turns of the ring
 #pragma unroll 1
-  for (int i = 0; i < count; ++i) {
-    if ((i & 31) == 0) {
-      if (i > 0) place = place_next;
-      base = i;
-      place_next = locate(i + 32 + lane);
-    }
-    if ((i & 31) == 8) load_scales(i - 8 + 32 + lane, place_next);
-    if ((i & 31) == 24) keep_scales(i - 24 + 32 + lane);
-    const int ahead = i + S::kStages - 1;
-    issue(ahead, stage == 0 ? S::kStages - 1 : stage - 1);
-    cp_async_wait<S::kStages - 1>();
-    __syncwarp();
-    const uint8_t* kt = ring + stage * S::kStageBytes;
-    const uint8_t* vt = kt + 16 * D;
-
-    // ---- scores: c[0..1] token g of rows 2 tq, 2 tq + 1; c[2..3] token g + 8
-    float sc[NT][4];
+  for (; base < count; base += 32) {
+    if (base > 0) place = place_next;
+    place_next = locate(base + 32 + lane);
+#pragma unroll 1
+    for (int i0 = base; i0 < min(base + 32, count); i0 += S::kStages) {
+      if (i0 - base == 8) load_scales(base + 32 + lane, place_next);
+      if (i0 - base == 24) keep_scales(base + 32 + lane);
+      const float4* mt = meta + (i0 & 63);
+      const int tok0 = (first + warps * i0) * 16;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sc[nt][e] = 0.f;
-#pragma unroll
-    for (int c = 0; c < (S::kSteps + 3) / 4; ++c) {
-      uint32_t w[2][4];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (c < D / 64) {
-          const uint4 v = *reinterpret_cast<const uint4*>(kt + tile_offset<D>(krow + 8 * h, c * 64 + tq * 16));
-          w[h][0] = v.x; w[h][1] = v.y; w[h][2] = v.z; w[h][3] = v.w;
-        } else {
-#pragma unroll
-          for (int j = 0; j < S::kSteps - 4 * c && j < 4; ++j)
-            w[h][j] = *reinterpret_cast<const uint32_t*>(kt + tile_offset<D>(krow + 8 * h, c * 64 + j * 16 + tq * 4));
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int s = 4 * c + j;
-        if (s < S::kSteps) {
-          const uint32_t a[4] = {codes_to_half2(w[0][j]), codes_to_half2(w[1][j]), codes_to_half2(w[0][j] >> 8),
-                                 codes_to_half2(w[1][j] >> 8)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int term = 0; term < S::kTerms; ++term) {
-              if (S::kQueryInSmem) {
-                const uint2 b = q_smem[((term * NT + nt) * S::kSteps + s) * 32 + lane];
-                mma_half(sc[nt], a, b.x, b.y);
-              } else {
-                const auto& b = qb[S::kQueryInSmem ? 0 : nt][S::kQueryInSmem ? 0 : s][term];
-                mma_half(sc[nt], a, b[0], b[1]);
-              }
-            }
+      for (int st = 0; st < S::kStages; ++st) {
+        if (i0 + st < count) {
+          issue(i0 + st + S::kStages - 1, (st + S::kStages - 1) % S::kStages);
+          cp_async_wait<S::kStages - 1>();
+          __syncwarp();
+          sum.tile(ring + st * S::kStageBytes, ring_u32 + st * S::kStageBytes + 16 * D, mt[st],
+                   tok0 + st * (warps * 16), query, ln);
+          __syncwarp();  // every lane is done with the stage before it is filled again
         }
       }
     }
-
-    // ---- weights
-    const float4 mt = meta[i & 63];
-    const int tok0 = (first + kWarps * i) * 16;
-    const bool partial = tok0 + 16 > vis_all;
-    uint32_t pb[NT][S::kTerms][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float mul[2] = {mt.x * s_mul[nt][0], mt.x * s_mul[nt][1]};
-      float x[4];  // base-2 exponents against the running maximum
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = fmaf(sc[nt][e], mul[e & 1], mt.y - m_run[nt][e & 1]);
-      if (partial) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (tok0 + krow + 8 * (e >> 1) >= vis[nt][e & 1]) x[e] = -INFINITY;
-      }
-      // NaN - as for a row that has no maximum yet - compares false: such rows come here too
-      const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-      if (__any_sync(0xffffffffu, !(top <= kRescaleSlack))) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float y0 = tok0 + krow < vis[nt][e] ? fmaf(sc[nt][e], mul[e], mt.y) : -INFINITY;
-          const float y1 = tok0 + krow + 8 < vis[nt][e] ? fmaf(sc[nt][e + 2], mul[e], mt.y) : -INFINITY;
-          float mx = fmaxf(y0, y1);
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          float& m = m_run[nt][e];
-          if (mx > m + kRescaleSlack) {
-            const float alpha = m == -INFINITY ? 0.f : exp2_approx(m - mx);
-            m = mx;
-            l_run[nt][e] *= alpha;
-#pragma unroll
-            for (int t = 0; t < S::kTiles; ++t) {
-              acc[nt][t][e] *= alpha;
-              acc[nt][t][e + 2] *= alpha;
-            }
-          }
-          // a row that has seen no token yet has m = -inf, and -inf - m would be a NaN
-          x[e] = y0 == -INFINITY ? -INFINITY : y0 - m;
-          x[e + 2] = y1 == -INFINITY ? -INFINITY : y1 - m;
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = exp2_approx(x[e]);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) l_run[nt][e] = fmaf(x[e] + x[e + 2], mt.z, l_run[nt][e]);
-#pragma unroll
-      for (int term = 0; term < S::kTerms; ++term) {
-        pb[nt][term][0] = transpose8(pack_half2(x[0], x[1]));
-        pb[nt][term][1] = transpose8(pack_half2(x[2], x[3]));
-        if (term + 1 < S::kTerms) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] -= __half2float(__float2half_rn(x[e]));
-        }
-      }
-    }
-
-    // ---- out^T += V^T w^T. `word`: 4 neighbouring dims (columns n .. n + 3) of the tokens
-    // tq, tq + 4, tq + 8, tq + 12
-    auto product = [&](uint32_t t0, uint32_t t1, uint32_t t2, uint32_t t3, int n) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int tile = n / 2 + half;
-        if (tile < S::kTiles) {
-          // two tokens side by side: (dim, dim + 1) of one, then of the other
-          const uint32_t lo = __byte_perm(t0, t1, half ? 0x7632 : 0x5410);
-          const uint32_t hi = __byte_perm(t2, t3, half ? 0x7632 : 0x5410);
-          const uint32_t a[4] = {codes_to_half2(lo), codes_to_half2(lo >> 8), codes_to_half2(hi), codes_to_half2(hi >> 8)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int term = 0; term < S::kTerms; ++term) mma_half(acc[nt][tile], a, pb[nt][term][0], pb[nt][term][1]);
-        }
-      }
-    };
-    constexpr int k16 = D / 128, k8 = (D % 128) / 64, k4 = (D % 64) / 32, k2 = (D % 32) / 16;
-#pragma unroll
-    for (int c = 0; c < k16; ++c) {
-      uint4 v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const uint4*>(vt + tile_offset<D>(tq + 4 * e, c * 128 + g * 16));
-      product(v[0].x, v[1].x, v[2].x, v[3].x, 16 * c);
-      product(v[0].y, v[1].y, v[2].y, v[3].y, 16 * c + 4);
-      product(v[0].z, v[1].z, v[2].z, v[3].z, 16 * c + 8);
-      product(v[0].w, v[1].w, v[2].w, v[3].w, 16 * c + 12);
-    }
-    if (k8) {
-      constexpr int b = k16 * 128;
-      uint2 v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const uint2*>(vt + tile_offset<D>(tq + 4 * e, b + g * 8));
-      product(v[0].x, v[1].x, v[2].x, v[3].x, b / 8);
-      product(v[0].y, v[1].y, v[2].y, v[3].y, b / 8 + 4);
-    }
-    if (k4) {
-      constexpr int b = k16 * 128 + k8 * 64;
-      uint32_t v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const uint32_t*>(vt + tile_offset<D>(tq + 4 * e, b + g * 4));
-      product(v[0], v[1], v[2], v[3], b / 8);
-    }
-    if (k2) {
-      constexpr int b = k16 * 128 + k8 * 64 + k4 * 32;
-      uint32_t v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const uint16_t*>(vt + tile_offset<D>(tq + 4 * e, b + g * 2));
-      product(v[0], v[1], v[2], v[3], b / 8);
-    }
-    stage = stage + 1 == S::kStages ? 0 : stage + 1;
-    __syncwarp();  // every lane is done with the stage before it is filled again
   }
   cp_async_wait<0>();
 
   // ---- the warps' sums meet: m, l, acc per row, then one thread per (row, dim)
   __syncthreads();  // the rings are free
+  sum.reduce();
   float* sums = reinterpret_cast<float*>(smem);            // [warp][row][D]
-  float* ml = sums + kWarps * S::kRows * D;                // [warp][row][2]
-  float* cta_sum = ml + kWarps * S::kRows * 2;             // [row][D]
+  float* ml = sums + warps * S::kRows * D;                // [warp][row][2]
+  float* cta_sum = ml + warps * S::kRows * 2;             // [row][D]
   float* cta_ml = cta_sum + S::kRows * D;                  // [row][2]
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float l = l_run[nt][e];
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      const int row = nt * 8 + 2 * tq + e;
+      const int row = nt * 8 + 2 * ln.tq + e;
       if (row < nrows) {
-        if (g == 0) *reinterpret_cast<float2*>(ml + (warp * S::kRows + row) * 2) = make_float2(m_run[nt][e], l);
+        if (ln.g == 0)
+          *reinterpret_cast<float2*>(ml + (warp * S::kRows + row) * 2) = make_float2(sum.m[nt][e], sum.l[nt][e]);
         float* dst = sums + (warp * S::kRows + row) * D;
 #pragma unroll
         for (int t = 0; t < S::kTiles; ++t) {
-          dst[v_dim<D>(2 * t, g)] = acc[nt][t][e];
-          dst[v_dim<D>(2 * t + 1, g)] = acc[nt][t][e + 2];
+          dst[16 * t + ln.g] = sum.acc[nt][t][e];
+          dst[16 * t + ln.g + 8] = sum.acc[nt][t][e + 2];
         }
       }
     }
@@ -597,14 +657,12 @@ __global__ void __launch_bounds__(kThreads) paged_attention_int8_kernel(const In
       if (d == 0) p.ws_ml[item] = make_float2(m, l);
     }
   };
-  for (int i = threadIdx.x; i < nrows * D; i += kThreads) {
+  for (int i = threadIdx.x; i < nrows * D; i += blockDim.x) {
     const int row = i / D, d = i - row * D;
     float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[(w * S::kRows + row) * 2]);
+    for (int w = 0; w < warps; ++w) m = fmaxf(m, ml[(w * S::kRows + row) * 2]);
     float l = 0.f, o = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < warps; ++w) {
       const float f = merge_factor(ml[(w * S::kRows + row) * 2], m);
       l = fmaf(f, ml[(w * S::kRows + row) * 2 + 1], l);
       o = fmaf(f, sums[(w * S::kRows + row) * D + d], o);
@@ -622,7 +680,7 @@ __global__ void __launch_bounds__(kThreads) paged_attention_int8_kernel(const In
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
   const int rank = split % p.cluster;
-  for (int i = rank * kThreads + threadIdx.x; i < nrows * D; i += p.cluster * kThreads) {
+  for (int i = rank * blockDim.x + threadIdx.x; i < nrows * D; i += p.cluster * blockDim.x) {
     const int row = i / D, d = i - row * D;
     float m = -INFINITY;
     float2 part[kMaxCluster];
@@ -676,6 +734,13 @@ __global__ void combine_int8_kernel(const Int8AttnParams p, int D) {
   }
 }
 
+// Dynamic shared memory of a CTA, as the kernel lays it out.
+int smem_bytes(int dtype, int D, int rows, int warps) {
+  const int ring = warps * 32 * D * (D <= 128 ? 4 : 2), merge = (warps + 1) * rows * (D + 2) * 4;
+  const int words = (dtype == VFL_DTYPE_F32 ? 3 : 2) * rows / 8 * (D / 16);
+  return (ring > merge ? ring : merge) + warps * 64 * 16 + (words > 32 ? words * 128 : 0);
+}
+
 int64_t acc_bytes(int64_t items, int D) { return ceil_div(items * D * 4, (int64_t)256) * 256; }
 
 int64_t workspace_of(const vfl_attention_int8_plan* plan) {
@@ -689,21 +754,34 @@ int64_t row_chunks(const vfl_attention_int8_plan* plan) {
   return ceil_div((int64_t)plan->max_q_len * (plan->num_heads / plan->num_kv_heads), (int64_t)plan->rows_per_cta);
 }
 
+// About `splits` CTAs a context: a power of two up to a cluster's 8, multiples of 8 past it.
+void set_splits(vfl_attention_int8_plan* plan, int64_t splits) {
+  int cluster = 1;
+  while (cluster < kMaxCluster && 2 * cluster <= splits) cluster *= 2;
+  plan->cluster = cluster;
+  plan->num_splits = static_cast<int32_t>(cluster < kMaxCluster ? cluster : splits / kMaxCluster * kMaxCluster);
+}
+
 // Whether 16 query rows a CTA are built: past 128 dims their sums do not fit the registers.
 bool rows16_built(int head_dim) { return head_dim <= 128; }
 
+struct Launch {
+  dim3 grid;
+  int threads, smem;
+  cudaStream_t stream;
+};
+
 template <typename T, int D, int NT>
-int launch(const Int8AttnParams& p, dim3 grid, cudaStream_t stream) {
+int launch(const Int8AttnParams& p, const Launch& l) {
   static int smem_done[kMaxDevices] = {};
   auto kern = paged_attention_int8_kernel<T, D, NT>;
-  constexpr int kSmem = Shape<T, D, NT>::kSmem;
-  const int st = ensure_smem_attribute(reinterpret_cast<const void*>(kern), kSmem, smem_done);
+  const int st = ensure_smem_attribute(reinterpret_cast<const void*>(kern), l.smem, smem_done);
   if (st) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = stream;
+  cfg.gridDim = l.grid;
+  cfg.blockDim = dim3(l.threads, 1, 1);
+  cfg.dynamicSmemBytes = l.smem;
+  cfg.stream = l.stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
@@ -715,39 +793,32 @@ int launch(const Int8AttnParams& p, dim3 grid, cudaStream_t stream) {
 }
 
 template <typename T, int NT>
-int launch_dim(const Int8AttnParams& p, int D, dim3 grid, cudaStream_t s) {
+int launch_dim(const Int8AttnParams& p, int D, const Launch& l) {
   switch (D) {
-    case 32: return launch<T, 32, NT>(p, grid, s);
-    case 48: return launch<T, 48, NT>(p, grid, s);
-    case 64: return launch<T, 64, NT>(p, grid, s);
-    case 80: return launch<T, 80, NT>(p, grid, s);
-    case 96: return launch<T, 96, NT>(p, grid, s);
-    case 112: return launch<T, 112, NT>(p, grid, s);
-    case 128: return launch<T, 128, NT>(p, grid, s);
+    case 32: return launch<T, 32, NT>(p, l);
+    case 48: return launch<T, 48, NT>(p, l);
+    case 64: return launch<T, 64, NT>(p, l);
+    case 80: return launch<T, 80, NT>(p, l);
+    case 96: return launch<T, 96, NT>(p, l);
+    case 112: return launch<T, 112, NT>(p, l);
+    case 128: return launch<T, 128, NT>(p, l);
     default: break;
   }
   if constexpr (NT == 1) {
     switch (D) {
-      case 160: return launch<T, 160, 1>(p, grid, s);
-      case 192: return launch<T, 192, 1>(p, grid, s);
-      case 224: return launch<T, 224, 1>(p, grid, s);
-      case 256: return launch<T, 256, 1>(p, grid, s);
-      default: return launch<T, 512, 1>(p, grid, s);
+      case 160: return launch<T, 160, 1>(p, l);
+      case 192: return launch<T, 192, 1>(p, l);
+      case 224: return launch<T, 224, 1>(p, l);
+      case 256: return launch<T, 256, 1>(p, l);
+      default: return launch<T, 512, 1>(p, l);
     }
   }
   return fail(VFL_ERR_UNSUPPORTED, "attention_int8: 16 rows a CTA at head_dim %d", D);
 }
 
 template <typename T>
-int launch_rows(const Int8AttnParams& p, int D, int rows, dim3 grid, cudaStream_t s) {
-  return rows == 16 ? launch_dim<T, 2>(p, D, grid, s) : launch_dim<T, 1>(p, D, grid, s);
-}
-
-// Dynamic shared memory of a CTA (upper bound over the types).
-int smem_bytes(int D, int rows) {
-  const int ring = kWarps * 32 * D * (D <= 128 ? 4 : (D <= 256 ? 3 : 2));
-  const int merge = (kWarps + 1) * rows * (D + 2) * 4;
-  return (ring > merge ? ring : merge) + kWarps * 64 * 16 + (2 * rows * D > 1024 ? 4 * rows * D : 0);
+int launch_rows(const Int8AttnParams& p, int D, int rows, const Launch& l) {
+  return rows == 16 ? launch_dim<T, 2>(p, D, l) : launch_dim<T, 1>(p, D, l);
 }
 
 // A plan is caller memory: what the kernels rely on is checked again.
@@ -767,6 +838,9 @@ int check_plan(const vfl_attention_int8_plan* plan) {
     return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: plan splits %d in clusters of %d", plan->num_splits, c);
   if (!(plan->rows_per_cta == 8 || (plan->rows_per_cta == 16 && rows16_built(plan->head_dim))))
     return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: plan rows_per_cta %d", plan->rows_per_cta);
+  if (!(plan->warps == 1 || plan->warps == 2 || plan->warps == 4 || plan->warps == kMaxWarps) ||
+      smem_bytes(plan->dtype, plan->head_dim, plan->rows_per_cta, plan->warps) > kSmemPerSM)
+    return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: plan warps %d", plan->warps);
   if (row_chunks(plan) > 65535 || (int64_t)plan->num_reqs * plan->num_kv_heads > INT32_MAX ||
       plan->max_q_len > 65535 || plan->num_heads > 65535)
     return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: plan launch grid too large");
@@ -828,25 +902,38 @@ int vfl_plan_attention_int8(int num_reqs, int num_heads, int num_kv_heads, int h
   }
 
   // Splits: as many as give every CTA slot an item, each of at least a tile a warp.
-  int per_sm = kSmemPerSM / (smem_bytes(head_dim, plan->rows_per_cta) + 1024);
+  plan->warps = 4;
+  int per_sm = kSmemPerSM / (smem_bytes(dtype, head_dim, plan->rows_per_cta, plan->warps) + 1024);
   per_sm = per_sm < 1 ? 1 : (per_sm > 4 ? 4 : per_sm);
   const int64_t slots = (int64_t)kNumSMs * per_sm;
   const int64_t tiles = ceil_div(max_seq, (int64_t)16);
   int64_t splits = 1;
   if (items > 0) {
-    const int64_t by_len = tiles / kWarps;
+    const int64_t by_len = tiles / plan->warps;
     splits = slots / items;
     splits = splits < by_len ? splits : by_len;
   }
-  int cluster = 1;
-  while (cluster < kMaxCluster && 2 * cluster <= splits) cluster *= 2;
-  plan->cluster = cluster;
-  plan->num_splits = static_cast<int32_t>(cluster < kMaxCluster ? cluster : splits / kMaxCluster * kMaxCluster);
+  set_splits(plan, splits);
   plan->workspace_bytes = workspace_of(plan);
   plan->magic = VFL_INT8_PLAN_MAGIC;
   st = check_plan(plan);
   if (st) plan->magic = 0;
   return st;
+}
+
+int vfl_plan_attention_int8_shape(vfl_attention_int8_plan* plan, int warps, int num_splits) {
+  int st = check_plan(plan);
+  if (st) return st;
+  vfl_attention_int8_plan next = *plan;
+  if (warps != 0) next.warps = warps;
+  if (num_splits < 0 || num_splits > 65535)
+    return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: num_splits %d", num_splits);
+  if (num_splits > 0) set_splits(&next, num_splits);
+  next.workspace_bytes = workspace_of(&next);
+  st = check_plan(&next);
+  if (st) return st;
+  *plan = next;
+  return VFL_OK;
 }
 
 int vfl_attention_with_kv_cache_int8(const vfl_attention_int8_plan* plan, const void* query, int64_t query_token_stride,
@@ -872,15 +959,15 @@ int vfl_attention_with_kv_cache_int8(const vfl_attention_int8_plan* plan, const 
   if (query_token_stride < (int64_t)H * D || output_token_stride < (int64_t)H * D)
     return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: token stride smaller than a token");
   if (!aligned16(query) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(output) ||
-      (query_token_stride * es) % 16 != 0)
-    return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: tensors and the query stride must be 16-byte aligned");
+      (query_token_stride * es) % 16 != 0 || (output_token_stride * es) % 16 != 0)
+    return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: tensors and token strides must be 16-byte aligned");
   if (!(scale == scale) || fabsf(scale) > FLT_MAX)
     return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: scale is not finite");
   if (plan->workspace_bytes > 0 &&
       (workspace == nullptr || !aligned16(workspace) || workspace_bytes < (size_t)plan->workspace_bytes))
     return fail(VFL_ERR_WORKSPACE, "attention_int8: needs %lld workspace bytes (16-byte aligned), got %zu",
                 (long long)plan->workspace_bytes, workspace_bytes);
-  Int8AttnParams p;
+  Int8AttnParams p = {};
   st = device_error_word(&p.err);
   if (st) return st;
   p.q = query;
@@ -912,9 +999,13 @@ int vfl_attention_with_kv_cache_int8(const vfl_attention_int8_plan* plan, const 
   p.ws_ml = clusters > 1
                 ? reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + acc_bytes(items, D)) : nullptr;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(plan->num_reqs * plan->num_kv_heads, (unsigned)row_chunks(plan), plan->num_splits);
-  st = plan->dtype == VFL_DTYPE_F32 ? launch_rows<float>(p, D, plan->rows_per_cta, grid, s)
-                                    : launch_rows<__nv_bfloat16>(p, D, plan->rows_per_cta, grid, s);
+  Launch l;
+  l.grid = dim3(plan->num_reqs * plan->num_kv_heads, (unsigned)row_chunks(plan), plan->num_splits);
+  l.threads = plan->warps * 32;
+  l.smem = smem_bytes(plan->dtype, D, plan->rows_per_cta, plan->warps);
+  l.stream = s;
+  st = plan->dtype == VFL_DTYPE_F32 ? launch_rows<float>(p, D, plan->rows_per_cta, l)
+                                    : launch_rows<__nv_bfloat16>(p, D, plan->rows_per_cta, l);
   if (st || clusters == 1) return st;
   const dim3 cgrid(plan->num_reqs, plan->max_q_len, H);
   const int threads = D <= 64 ? 64 : 128;

@@ -737,6 +737,15 @@ def plan_of_int8(metadata: torch.Tensor) -> N.AttentionInt8Plan:
     return plan
 
 
+def set_shape_int8(metadata: torch.Tensor, warps: int = 0, num_splits: int = 0) -> torch.Tensor:
+    """Re-plan ``metadata`` (in place) for CTAs of ``warps`` (1, 2, 4, 8) warps and about
+    ``num_splits`` CTAs a context (0: as planned); returns it. ``ValueError`` where not built."""
+    st = N.lib().vfl_plan_attention_int8_shape(ctypes.byref(plan_of_int8(metadata)), int(warps), int(num_splits))
+    if st != N.VFL_OK:
+        raise ValueError(f"vflorence_b200: {N.last_error()}")
+    return metadata
+
+
 def attention_with_kv_cache_int8(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                                  k_scale: torch.Tensor, v_scale: torch.Tensor, output: torch.Tensor,
                                  query_start_loc: torch.Tensor, seq_lens: torch.Tensor, scale: float, causal: bool,
