@@ -402,7 +402,7 @@ typedef struct vfl_attention_int8_plan {
   int32_t rows_per_cta;    /* query rows (tokens x heads of a K/V head) a CTA takes: 8 or 16 */
   int32_t num_splits;      /* CTAs that share a context                                      */
   int32_t cluster;         /* of them in a thread-block cluster: 1, 2, 4 or 8                */
-  int32_t warps;           /* of a CTA, each with tiles of its own: 1, 2, 4 or 8             */
+  int32_t warps;           /* of a CTA, each with tiles of its own: 1, 2 or 4                */
   int64_t workspace_bytes; /* scratch the caller must pass (0 = none)                        */
 } vfl_attention_int8_plan;
 

@@ -267,9 +267,9 @@ def attention_exact(q, cache, qsl, lens, table, scale, causal):
     return out, top
 
 
-@pytest.fixture(params=[0, 1, 8])
+@pytest.fixture(params=[0, 1, 2, 4])
 def warps(request):
-    """Warps a CTA: as planned, and the fewest and most."""
+    """Warps a CTA: as planned, and each count."""
     return request.param
 
 
@@ -279,10 +279,7 @@ def attend(warps, q, cache, qsl, lens, table, scale, causal, planned=None, out=N
                                            lens if planned is None else planned, q.dtype, qsl, causal,
                                            cache[0].shape[2])
     if warps:
-        try:
-            ops.set_shape_int8(meta, warps)
-        except ValueError:
-            pytest.skip("rings of 8 warps do not fit at this head_dim")
+        ops.set_shape_int8(meta, warps)
     qd = q.cuda()
     out = torch.full_like(qd, 7.0) if out is None else out
     ops.attention_with_kv_cache_int8(qd, *dev, out, qsl.cuda(), lens.cuda(), scale, causal, table.cuda(), meta)
@@ -350,7 +347,7 @@ def test_attention_block_sizes_and_splits(warps, bs, dtype):
     q, cache, qsl, lens, table = batch([1500, 1, 400, 17], [2, 1, 1, 3], 2, 1, 64, bs, dtype, seed=bs)
     want, top = attention_exact(q, cache, qsl, lens, table, 0.125, False)
     got, plan = attend(warps, q, cache, qsl, lens, table, 0.125, False)
-    assert plan.num_splits > plan.cluster
+    assert plan.num_splits > 1
     assert_close(got, want, top, dtype)
 
 

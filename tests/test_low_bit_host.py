@@ -91,11 +91,11 @@ def test_attention_refuses_bad_arguments(native):
                 dict(o_stride=256), dict(t_stride=4), dict(kc=PTR + 1), dict(query=PTR + 8),
                 dict(scale=float("nan")), dict(scale=float("inf"))):
         assert _attend(native, plan, **bad) == 1, bad
-    split_meta = _plan([9000], heads=8, kv=8, d=64)
+    split_meta = _plan([20000], heads=8, kv=8, d=64)
     split = ops.plan_of_int8(split_meta)
     assert split.workspace_bytes > 0
-    assert _attend(native, split, cols=600, t_stride=600) == 3
-    assert _attend(native, split, cols=600, t_stride=600, ws=PTR, ws_bytes=16) == 3
+    assert _attend(native, split, cols=1300, t_stride=1300) == 3
+    assert _attend(native, split, cols=1300, t_stride=1300, ws=PTR, ws_bytes=16) == 3
     empty = _plan([], heads=4, kv=4)
     assert _attend(native, ops.plan_of_int8(empty)) == 0
 

@@ -42,7 +42,7 @@ namespace cg = cooperative_groups;
 namespace vfl {
 namespace {
 
-constexpr int kMaxWarps = 8;
+constexpr int kMaxWarps = 4;
 constexpr int kMaxCluster = 8;
 constexpr int kSmemPerSM = 227 * 1024;
 constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: smaller V scales count as it
@@ -177,6 +177,8 @@ struct Shape {
   static constexpr int kStageBytes = 2 * 16 * D;
   static constexpr int kStages = D <= 128 ? 4 : 2;
   static constexpr int kRingBytes = kStages * kStageBytes;
+  // CTAs of four warps that an SM's registers are to hold (96, 128 and 168 a lane)
+  static constexpr int kMinCtas = D * NT <= 64 ? 5 : (D * NT <= 128 ? (sizeof(T) == 4 ? 3 : 4) : (D <= 128 ? 2 : 1));
   // query digits stay in registers up to this many, in shared memory past it
   static constexpr bool kQueryInSmem = kPlanes * NT * kWords > 32;
   // the warps' rings, later their sums [warp][row][D], the CTA's [row][D] and all their (m, l)
@@ -205,6 +207,19 @@ __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, flo
 __device__ __forceinline__ void store_elem(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_elem(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+__device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+  *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+}
+__device__ __forceinline__ void add_scaled(float4& o, float f, const float4& v) {
+  o.x = fmaf(f, v.x, o.x);
+  o.y = fmaf(f, v.y, o.y);
+  o.z = fmaf(f, v.z, o.z);
+  o.w = fmaf(f, v.w, o.w);
+}
+
 // Factor of a piece with maximum `m` in a sum with maximum `m_all`. A piece without a maximum
 // holds zeros (nothing visible) or NaNs (every score a NaN), and either is to be kept.
 __device__ __forceinline__ float merge_factor(float m, float m_all) {
@@ -220,6 +235,9 @@ __device__ __forceinline__ int k_dim(int w, int tq) {
   if (w < 4 * k64 + 2 * k32) return k64 * 64 + tq * 8 + (w - 4 * k64) * 4;
   return k64 * 64 + k32 * 32 + tq * 4;
 }
+
+// 2^e for e in [-126, 127].
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // A lane's place in the fragments.
 struct Lane {
@@ -287,9 +305,10 @@ struct Query {
       // 2^e > amax >= 2^(e-1), from the exponent bits
       const int e = max(-90, static_cast<int>(__float_as_uint(amax) >> 23) - 126);
       constexpr int kBits = S::kPlanes == 3 ? 22 : 14;
-      const float to_int = ldexpf(1.f, kBits - e);
+      const float to_int = power_of_two(kBits - e);
 #pragma unroll
       for (int w = 0; w < S::kWords; ++w) {
+        if (S::kQueryInSmem && w % warps != warp) continue;
         float(&v)[4] = f[w < kHeld ? w : 0];
         if (kHeld == 1) {
           v[0] = v[1] = v[2] = v[3] = 0.f;
@@ -309,14 +328,14 @@ struct Query {
           }
           const int at = (nt * S::kPlanes + plane) * S::kWords + w;
           if (S::kQueryInSmem) {
-            if (w % warps == warp) q_smem[at * 32 + ln.lane] = packed;
+            q_smem[at * 32 + ln.lane] = packed;
           } else {
             digits[S::kQueryInSmem ? 0 : at] = packed;
           }
         }
       }
       // a row with an infinity or a NaN scores NaN
-      const float row_mul = bad ? NAN : ldexpf(p.scale_log2, e - kBits);
+      const float row_mul = bad ? NAN : p.scale_log2 * power_of_two(e - kBits);
 #pragma unroll
       for (int e2 = 0; e2 < 2; ++e2) {
         mul[nt][e2] = __shfl_sync(0xffffffffu, row_mul, (2 * ln.tq + e2) * 4);
@@ -490,7 +509,7 @@ struct Sums {
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kMaxWarps * 32) paged_attention_int8_kernel(const Int8AttnParams p) {
+__global__ void __launch_bounds__(kMaxWarps * 32, Shape<T, D, NT>::kMinCtas) paged_attention_int8_kernel(const Int8AttnParams p) {
   using S = Shape<T, D, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   const Lane ln;
@@ -500,6 +519,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32) paged_attention_int8_kernel(co
   const int split = blockIdx.z;
   const int bs = p.block_size, tpb = bs >> 4;
   const RequestSpan req = request_span(p, r);
+  // an unsplit context's first tiles do not depend on its length: their table entries come with it
+  const int32_t* table = p.table + (int64_t)r * p.table_stride;
+  int entry = 0;
+  if (p.num_splits == 1) {
+    const int col = (warp + warps * lane) / tpb;
+    if (col < p.table_cols) entry = __ldg(table + col);
+  }
   if (req.rows < 0) {
     if (threadIdx.x == 0 && kvh == 0 && blockIdx.y == 0 && split == 0) report(p.err, VFL_DEVERR_QUERY);
     return;
@@ -524,18 +550,18 @@ __global__ void __launch_bounds__(kMaxWarps * 32) paged_attention_int8_kernel(co
   // 32 tiles in units of 16 tokens of the pools, and of the next 32.
   const int first = tile_begin + warp;
   const int count = tile_end > first ? ceil_div(tile_end - first, warps) : 0;
-  auto locate = [&](int i) {
+  auto locate = [&](int i, bool have_entry) {
     if (i >= count) return 0;
     const int tile = first + warps * i;
     const int col = tpb == 1 ? tile : tile / tpb;
-    int b = __ldg(p.table + (int64_t)r * p.table_stride + col);
+    int b = have_entry ? entry : __ldg(table + col);
     if (b < 0 || b >= p.num_blocks) {
       report(p.err, VFL_DEVERR_BLOCK_ID);
       b = 0;
     }
     return (b * p.num_kv_heads + kvh) * tpb + (tile - col * tpb);  // the host checked that it fits
   };
-  int place = locate(lane), place_next = 0;
+  int place = locate(lane, p.num_splits == 1), place_next = 0;
   uint8_t* ring = smem + warp * S::kRingBytes;
   const uint32_t ring_u32 = smem_u32(ring);
   // where this lane's 16-byte pieces of a tile go, within a stage
@@ -597,7 +623,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32) paged_attention_int8_kernel(co
 #pragma unroll 1
   for (; base < count; base += 32) {
     if (base > 0) place = place_next;
-    place_next = locate(base + 32 + lane);
+    place_next = locate(base + 32 + lane, false);
 #pragma unroll 1
     for (int i0 = base; i0 < min(base + 32, count); i0 += S::kStages) {
       if (i0 - base == 8) load_scales(base + 32 + lane, place_next);
@@ -623,9 +649,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32) paged_attention_int8_kernel(co
   __syncthreads();  // the rings are free
   sum.reduce();
   float* sums = reinterpret_cast<float*>(smem);            // [warp][row][D]
-  float* ml = sums + warps * S::kRows * D;                // [warp][row][2]
-  float* cta_sum = ml + warps * S::kRows * 2;             // [row][D]
-  float* cta_ml = cta_sum + S::kRows * D;                  // [row][2]
+  float* cta_sum = sums + warps * S::kRows * D;            // [row][D]
+  float* ml = cta_sum + S::kRows * D;                      // [warp][row][2]
+  float* cta_ml = ml + warps * S::kRows * 2;               // [row][2]
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -644,65 +670,80 @@ __global__ void __launch_bounds__(kMaxWarps * 32) paged_attention_int8_kernel(co
     }
   __syncthreads();
   const int clusters = p.num_splits / p.cluster;
-  auto finish = [&](int row, int d, float m, float l, float o) {
+  // one row's sums, four dims a lane: the output, or the cluster's piece
+  auto finish = [&](int row, float m, float l, auto&& sum_at) {
     const int vrow = row0 + row, token = vrow / group;
     const int64_t out_row = req.q_begin + token;
     const int head = kvh * group + vrow - token * group;
     if (clusters == 1) {
+      T* dst = static_cast<T*>(p.out) + out_row * p.out_stride + (int64_t)head * D;
       // l is a NaN where a score was: the row then is one, as in a plain softmax
-      store_elem(static_cast<T*>(p.out) + out_row * p.out_stride + (int64_t)head * D + d, l == 0.f ? 0.f : o / l);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      for (int d = lane * 4; d < D; d += 128) {
+        const float4 o = sum_at(d);
+        store4(dst + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+      }
     } else {
       const int64_t item = (out_row * p.num_heads + head) * clusters + split / p.cluster;
-      p.ws_acc[item * D + d] = o;
-      if (d == 0) p.ws_ml[item] = make_float2(m, l);
+      for (int d = lane * 4; d < D; d += 128) *reinterpret_cast<float4*>(p.ws_acc + item * D + d) = sum_at(d);
+      if (lane == 0) p.ws_ml[item] = make_float2(m, l);
     }
   };
-  for (int i = threadIdx.x; i < nrows * D; i += blockDim.x) {
-    const int row = i / D, d = i - row * D;
-    float m = -INFINITY;
-    for (int w = 0; w < warps; ++w) m = fmaxf(m, ml[(w * S::kRows + row) * 2]);
-    float l = 0.f, o = 0.f;
-    for (int w = 0; w < warps; ++w) {
-      const float f = merge_factor(ml[(w * S::kRows + row) * 2], m);
-      l = fmaf(f, ml[(w * S::kRows + row) * 2 + 1], l);
-      o = fmaf(f, sums[(w * S::kRows + row) * D + d], o);
-    }
+  for (int row = warp; row < nrows; row += warps) {
+    float m = -INFINITY, l = 0.f, f[kMaxWarps];
+#pragma unroll
+    for (int w = 0; w < kMaxWarps; ++w)
+      if (w < warps) m = fmaxf(m, ml[(w * S::kRows + row) * 2]);
+#pragma unroll
+    for (int w = 0; w < kMaxWarps; ++w)
+      if (w < warps) {
+        f[w] = merge_factor(ml[(w * S::kRows + row) * 2], m);
+        l = fmaf(f[w], ml[(w * S::kRows + row) * 2 + 1], l);
+      }
+    auto sum_at = [&](int d) {
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kMaxWarps; ++w)
+        if (w < warps) add_scaled(o, f[w], *reinterpret_cast<const float4*>(sums + (w * S::kRows + row) * D + d));
+      return o;
+    };
     if (p.cluster == 1) {
-      finish(row, d, m, l, o);
+      finish(row, m, l, sum_at);
     } else {
-      cta_sum[i] = o;
-      if (d == 0) *reinterpret_cast<float2*>(cta_ml + 2 * row) = make_float2(m, l);
+      for (int d = lane * 4; d < D; d += 128) *reinterpret_cast<float4*>(cta_sum + row * D + d) = sum_at(d);
+      if (lane == 0) *reinterpret_cast<float2*>(cta_ml + 2 * row) = make_float2(m, l);
     }
   }
   if (p.cluster == 1) return;
 
-  // ---- the cluster's sums meet: each CTA finishes a share of the (row, dim) pairs
+  // ---- the cluster's sums meet: each warp of the cluster finishes a share of the rows. The tiles'
+  // scales are done with: their place holds the factors of a row's pieces
+  float* row_factor = reinterpret_cast<float*>(smem + region);
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
-  const int rank = split % p.cluster;
-  for (int i = rank * blockDim.x + threadIdx.x; i < nrows * D; i += p.cluster * blockDim.x) {
-    const int row = i / D, d = i - row * D;
-    float m = -INFINITY;
-    float2 part[kMaxCluster];
-    float val[kMaxCluster];
+  for (int row = (split % p.cluster) * warps + warp; row < nrows; row += p.cluster * warps) {
+    float2 part = make_float2(-INFINITY, 0.f);  // lane c: of CTA c
+    if (lane < p.cluster) part = *reinterpret_cast<const float2*>(cluster.map_shared_rank(cta_ml, lane) + 2 * row);
+    float m = part.x;
 #pragma unroll
-    for (int c = 0; c < kMaxCluster; ++c) {
-      if (c < p.cluster) {
-        part[c] = *reinterpret_cast<const float2*>(cluster.map_shared_rank(cta_ml, c) + 2 * row);
-        val[c] = cluster.map_shared_rank(cta_sum, c)[i];
-        m = fmaxf(m, part[c].x);
-      }
-    }
-    float l = 0.f, o = 0.f;
+    for (int o = kMaxCluster / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = __shfl_sync(0xffffffffu, m, 0);
+    const float factor = lane < p.cluster ? merge_factor(part.x, m) : 0.f;
+    float l = lane < p.cluster ? factor * part.y : 0.f;
 #pragma unroll
-    for (int c = 0; c < kMaxCluster; ++c) {
-      if (c < p.cluster) {
-        const float f = merge_factor(part[c].x, m);
-        l = fmaf(f, part[c].y, l);
-        o = fmaf(f, val[c], o);
-      }
-    }
-    finish(row, d, m, l, o);
+    for (int o = kMaxCluster / 2; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    l = __shfl_sync(0xffffffffu, l, 0);
+    if (lane < kMaxCluster) row_factor[warp * kMaxCluster + lane] = factor;
+    __syncwarp();
+    finish(row, m, l, [&](int d) {
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int c = 0; c < p.cluster; ++c)
+        add_scaled(o, row_factor[warp * kMaxCluster + c],
+                   *reinterpret_cast<const float4*>(cluster.map_shared_rank(cta_sum, c) + row * D + d));
+      return o;
+    });
+    __syncwarp();
   }
   cluster.sync();  // no CTA leaves while another still reads its sums
 }
@@ -760,6 +801,40 @@ void set_splits(vfl_attention_int8_plan* plan, int64_t splits) {
   while (cluster < kMaxCluster && 2 * cluster <= splits) cluster *= 2;
   plan->cluster = cluster;
   plan->num_splits = static_cast<int32_t>(cluster < kMaxCluster ? cluster : splits / kMaxCluster * kMaxCluster);
+}
+
+// Warps and CTAs of an item. Measured on B200 (device time, bfloat16, head_dim 64; items = requests
+// x K/V heads x row chunks):
+//   * more items than slots: the CTA's start (about 5 us, five CTAs of four warps an SM) is spread
+//     over fewer warps. 8192 items of 9 tiles: 1, 2, 4 warps take 44, 53, 64 us; 4096 items of 32
+//     tiles: 63, 56, 60; 4096 of 128: 223, 187, 171. Hence one warp up to 16 tiles, two up to 64.
+//   * items that four warps run in little more than one wave, and two warps in one, run two (768
+//     items of 37 tiles: 16.6 against 20.5 us);
+//   * fewer items: the context is cut until the slots are full, over a cluster at most (one of 8
+//     takes 8.9 us for 16 items of 256 tiles, four clusters and the adding launch 10.1), past 512
+//     tiles over more.
+void choose_shape(vfl_attention_int8_plan* plan, int64_t items, int64_t tiles_sum) {
+  const int64_t mean = items > 0 ? tiles_sum / items : 0;
+  const int64_t longest = ceil_div((int64_t)plan->max_seq_len, (int64_t)16);
+  const int by_smem = kSmemPerSM / (smem_bytes(plan->dtype, plan->head_dim, plan->rows_per_cta, 4) + 1024);
+  const int lanes = plan->head_dim * plan->rows_per_cta;  // of a CTA's sums; see Shape::kMinCtas
+  const int by_regs = lanes <= 512 ? 5 : (lanes <= 1024 ? (plan->dtype == VFL_DTYPE_F32 ? 3 : 4) : 2);
+  const int per_sm = by_smem < 1 ? 1 : (by_smem < by_regs ? by_smem : by_regs);
+  const int64_t slots = (int64_t)kNumSMs * per_sm;  // of CTAs of four warps
+  plan->warps = 4;
+  int64_t splits = 1;
+  if (items > 2 * slots) {
+    plan->warps = mean <= 16 ? 1 : (mean <= 64 ? 2 : 4);
+  } else if (items > slots) {
+    plan->warps = mean <= 64 ? 2 : 4;
+  } else if (items > 0) {
+    splits = slots / items;
+    if (splits == 1 && 14 * items < 10 * slots && mean >= 64) splits = 2;
+    const int64_t by_len = ceil_div(longest, (int64_t)2 * plan->warps);
+    splits = splits < by_len ? splits : by_len;
+    if (longest <= 512 && splits > kMaxCluster) splits = kMaxCluster;
+  }
+  set_splits(plan, splits);
 }
 
 // Whether 16 query rows a CTA are built: past 128 dims their sums do not fit the registers.
@@ -838,7 +913,7 @@ int check_plan(const vfl_attention_int8_plan* plan) {
     return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: plan splits %d in clusters of %d", plan->num_splits, c);
   if (!(plan->rows_per_cta == 8 || (plan->rows_per_cta == 16 && rows16_built(plan->head_dim))))
     return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: plan rows_per_cta %d", plan->rows_per_cta);
-  if (!(plan->warps == 1 || plan->warps == 2 || plan->warps == 4 || plan->warps == kMaxWarps) ||
+  if (!(plan->warps == 1 || plan->warps == 2 || plan->warps == kMaxWarps) ||
       smem_bytes(plan->dtype, plan->head_dim, plan->rows_per_cta, plan->warps) > kSmemPerSM)
     return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: plan warps %d", plan->warps);
   if (row_chunks(plan) > 65535 || (int64_t)plan->num_reqs * plan->num_kv_heads > INT32_MAX ||
@@ -895,25 +970,15 @@ int vfl_plan_attention_int8(int num_reqs, int num_heads, int num_kv_heads, int h
   plan->max_seq_len = static_cast<int32_t>(max_seq);
 
   plan->rows_per_cta = max_q * group > 8 && rows16_built(head_dim) ? 16 : 8;
-  int64_t items = 0;
+  int64_t items = 0, tiles_sum = 0;
   for (int r = 0; r < num_reqs; ++r) {
     const int64_t ql = query_start_loc_host ? (int64_t)query_start_loc_host[r + 1] - query_start_loc_host[r] : 1;
-    if (seq_lens_host[r] > 0) items += ceil_div(ql * group, (int64_t)plan->rows_per_cta) * num_kv_heads;
+    const int64_t n = ceil_div(ql * group, (int64_t)plan->rows_per_cta) * num_kv_heads;
+    if (seq_lens_host[r] > 0) items += n;
+    tiles_sum += n * ceil_div((int64_t)seq_lens_host[r], (int64_t)16);
   }
 
-  // Splits: as many as give every CTA slot an item, each of at least a tile a warp.
-  plan->warps = 4;
-  int per_sm = kSmemPerSM / (smem_bytes(dtype, head_dim, plan->rows_per_cta, plan->warps) + 1024);
-  per_sm = per_sm < 1 ? 1 : (per_sm > 4 ? 4 : per_sm);
-  const int64_t slots = (int64_t)kNumSMs * per_sm;
-  const int64_t tiles = ceil_div(max_seq, (int64_t)16);
-  int64_t splits = 1;
-  if (items > 0) {
-    const int64_t by_len = tiles / plan->warps;
-    splits = slots / items;
-    splits = splits < by_len ? splits : by_len;
-  }
-  set_splits(plan, splits);
+  choose_shape(plan, items, tiles_sum);
   plan->workspace_bytes = workspace_of(plan);
   plan->magic = VFL_INT8_PLAN_MAGIC;
   st = check_plan(plan);

@@ -738,7 +738,7 @@ def plan_of_int8(metadata: torch.Tensor) -> N.AttentionInt8Plan:
 
 
 def set_shape_int8(metadata: torch.Tensor, warps: int = 0, num_splits: int = 0) -> torch.Tensor:
-    """Re-plan ``metadata`` (in place) for CTAs of ``warps`` (1, 2, 4, 8) warps and about
+    """Re-plan ``metadata`` (in place) for CTAs of ``warps`` (1, 2, 4) warps and about
     ``num_splits`` CTAs a context (0: as planned); returns it. ``ValueError`` where not built."""
     st = N.lib().vfl_plan_attention_int8_shape(ctypes.byref(plan_of_int8(metadata)), int(warps), int(num_splits))
     if st != N.VFL_OK:
