@@ -9,13 +9,19 @@
 // overflows, or large, where its rounding would shift the whole row. An entry of -inf (a
 // forbidden token) adds nothing. Bound: HBM, the row read once.
 //
-// One pass gives the sums and, in shared memory, the largest value of each lane's batch of 32
-// entries. The k-th largest of the threads' own maxima is a lower bound T of the k-th largest
-// entry (the maxima are distinct entries), so only batches whose maximum reaches T are read
-// again: about k of them, from L2. Their entries >= T are ranked by counting. Where ties at T
-// overflow the list (rows of mostly one value), T becomes the k-th best (value, index) pair and
-// the collection runs again. A row is cut over a cluster of up to 8 CTAs when there are few rows; the pieces meet in the first CTA's shared
-// memory.
+// One pass gives the sums and, in shared memory, the largest value of each thread's batches of four
+// 16-byte vectors. A value T is then taken that at least k, and not many more, of the threads' own
+// maxima reach: a lower bound of the k-th largest entry, since the maxima are distinct entries.
+// Only batches whose maximum reaches T, a few more than k, are read again, from L2; their entries
+// >= T are ranked by counting. (A bound from the first batches, with entries picked up as they
+// pass, reads nothing twice but collects six times as many: 58 us against 35 at 1024 x 51289,
+// k = 20.) Where ties at T overflow the list (rows of mostly one value), the bound becomes the k-th
+// best (value, index) pair of the threads' best entries and the collection runs again. A row is
+// cut over a cluster of up to 8 CTAs when there are few rows; the pieces meet in the first CTA's
+// shared memory.
+//
+// The pass is close to two other bounds: 1024 x 51289 bfloat16 entries are 11.5 a clock and SM at
+// the copy rate, the exponentials allow 16, and at about 6 instructions an entry the issue rate 21.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -27,10 +33,8 @@ namespace cg = cooperative_groups;
 namespace vfl {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxK = 64;
-constexpr int kMaxima = 2048;       // batch maxima kept per CTA; longer pieces fold batches together
+constexpr int kStages = 3;          // batches of a thread in flight
 constexpr int kCandidates = 1024;
 constexpr int kMaxCluster = 8;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -49,21 +53,43 @@ __device__ __forceinline__ uint64_t make_key(float v, uint32_t idx) {
   return ((uint64_t)ordered_bits(v + 0.f) << 32) | (uint32_t)~idx;
 }
 
-constexpr float kLowest = -150.f;  // e^-150 is 0 in float32, and so is its product with -150
+// Sums of a piece of a row: s = sum e^d, u = sum d e^d, d = x - m, where m is at most kSlack below
+// the largest entry. d is held above kFar: the term of an entry of -inf is 0, and not -inf * 0.
+constexpr float kSlack = 8.f, kFar = -1000.f;
 
-// Sums of a piece of a row against its maximum: s = sum e^(x - m), u = sum (x - m) e^(x - m).
+// Batches are summed in base 2 with one multiply-add an entry, t = x log2 e - r, r = m log2 e
+// rounded; what the rounding shifts all t by, at most 2^-8 for |m| below kRoom, is put right once
+// a batch. Entries are held at kLow, so that t stays finite. Batches of rows past kRoom go entry
+// by entry.
+constexpr float kLow = -1e38f, kRoom = 65536.f;
+
 struct Sums {
-  float m = -INFINITY, s = 0.f, u = 0.f;
-  bool nan = false;  // a NaN among the entries
+  float m, s, u;
+  bool nan;  // a NaN among the entries
+  __device__ __forceinline__ void reset() {
+    m = -INFINITY;
+    s = u = 0.f;
+    nan = false;
+  }
   __device__ __forceinline__ void raise(float m_new) {
     if (m_new > m) {
       if (m != -INFINITY) {
-        const float d = fmaxf(m - m_new, kLowest);
+        const float d = fmaxf(m - m_new, kFar);
         const float f = exp2_approx(d * kLog2eF);
         u = fmaf(s, d, u) * f;
         s *= f;
       }
       m = m_new;
+    }
+  }
+  __device__ __forceinline__ void add(float x) {
+    nan |= x != x;
+    if (x > m + kSlack) raise(x);
+    if (x != -INFINITY) {
+      const float d = fmaxf(x - m, kFar);
+      const float f = exp2_approx(d * kLog2eF);
+      s += f;
+      u = fmaf(d, f, u);
     }
   }
   __device__ __forceinline__ void merge(Sums o) {
@@ -73,6 +99,66 @@ struct Sums {
     o.raise(top);
     s += o.s;
     u += o.u;
+  }
+};
+
+// 16 bytes of a row.
+template <typename T>
+struct Vec;
+
+template <>
+struct Vec<float> {
+  static constexpr uint32_t kFill = 0xff800000u;  // -inf
+  // the largest entry, or a NaN if there is one
+  __device__ __forceinline__ static float max(const uint4& v) {
+    float m = __uint_as_float(v.x);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(v.y)));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(v.z)));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(v.w)));
+    return m;
+  }
+  template <typename F>
+  __device__ __forceinline__ static void each(const uint4& v, F&& f) {
+    f(__uint_as_float(v.x), 0);
+    f(__uint_as_float(v.y), 1);
+    f(__uint_as_float(v.z), 2);
+    f(__uint_as_float(v.w), 3);
+  }
+  // entries held at `low`
+  __device__ __forceinline__ static uint4 held(const uint4& v, float low) {
+    return make_uint4(__float_as_uint(fmaxf(__uint_as_float(v.x), low)), __float_as_uint(fmaxf(__uint_as_float(v.y), low)),
+                      __float_as_uint(fmaxf(__uint_as_float(v.z), low)), __float_as_uint(fmaxf(__uint_as_float(v.w), low)));
+  }
+};
+
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr uint32_t kFill = 0xff80ff80u;
+  __device__ __forceinline__ static __nv_bfloat162 two(uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+  __device__ __forceinline__ static float max(const uint4& v) {
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(two(v.x), two(v.y)), __hmax2_nan(two(v.z), two(v.w)));
+    float a = __low2float(m);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(__high2float(m)));
+    return a;
+  }
+  template <typename F>
+  __device__ __forceinline__ static void each(const uint4& v, F&& f) {
+    f(__uint_as_float(v.x << 16), 0);
+    f(__uint_as_float(v.x & 0xffff0000u), 1);
+    f(__uint_as_float(v.y << 16), 2);
+    f(__uint_as_float(v.y & 0xffff0000u), 3);
+    f(__uint_as_float(v.z << 16), 4);
+    f(__uint_as_float(v.z & 0xffff0000u), 5);
+    f(__uint_as_float(v.w << 16), 6);
+    f(__uint_as_float(v.w & 0xffff0000u), 7);
+  }
+  __device__ __forceinline__ static uint32_t held(uint32_t w, __nv_bfloat162 low) {
+    const __nv_bfloat162 x = __hmax2(two(w), low);
+    return *reinterpret_cast<const uint32_t*>(&x);
+  }
+  __device__ __forceinline__ static uint4 held(const uint4& v, float low) {
+    const __nv_bfloat162 l = __float2bfloat162_rn(low);
+    return make_uint4(held(v.x, l), held(v.y, l), held(v.z, l), held(v.w, l));
   }
 };
 
@@ -103,25 +189,76 @@ __device__ __forceinline__ float elem(const __nv_bfloat16* p) {
   return __uint_as_float((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p)) << 16);
 }
 
-struct Shared {
+// What the selection needs, in the place of the ring once the row has passed.
+template <int kThreads>
+struct Selection {
+  static constexpr int kMaxima = (kThreads < 512 ? 16 : 8) * kThreads;
   uint64_t keys[kCandidates];
   uint64_t best[kMaxCluster][kMaxK];  // of the pieces (used in the first CTA)
-  Sums part[kMaxCluster];
-  float maxima[kMaxima];
   uint64_t lane_key[kThreads];
-  int list[kMaxima];
-  Sums warp[kWarps];
-  int listed, found;
+  uint16_t list[kMaxima];
+};
+
+template <int kThreads>
+struct Shared {
+  union {
+    uint4 ring[kStages][4][kThreads];  // a thread reads what it copied itself
+    Selection<kThreads> sel;
+  };
+  // of the threads' batches, rounded up to 16 bits; longer pieces fold batches together
+  __nv_bfloat16 maxima[Selection<kThreads>::kMaxima];
+  uint32_t lane_max[kThreads];
+  Sums part[kMaxCluster];
+  Sums warp[kThreads / 32];
+  int listed, found, nan;
   uint64_t bound;
 };
 
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// A value that at least k of the threads' maxima reach, and where ties allow not many more: found
+// by halving, in one warp.
+template <int kThreads>
+__device__ __forceinline__ uint32_t value_bound(const uint32_t* maxima, int k, int lane) {
+  uint32_t v[kThreads / 32];
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) v[i] = maxima[i * 32 + lane];
+  uint32_t lo = v[0], hi = v[0];
+#pragma unroll
+  for (int i = 1; i < kThreads / 32; ++i) {
+    lo = min(lo, v[i]);
+    hi = max(hi, v[i]);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);  // every maximum reaches lo
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  // invariant: at least k reach lo, fewer than k reach hi + 1
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo + 1) / 2;
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) c += v[i] >= mid;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= k) {
+      lo = mid;
+      if (c <= k + k / 2 + 4) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  return lo;
+}
+
 // grid: rows x pieces, a cluster a row.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobParams p) {
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kernel(const LogprobParams p) {
   constexpr int N = Elem<T>::kVec;
-  constexpr int U = 32 / N;  // vectors of a lane's batch
+  constexpr int U = 4;  // vectors of a thread's batch
+  constexpr int kWarps = kThreads / 32, kMaxima = Selection<kThreads>::kMaxima;
+  using V = Vec<T>;
   extern __shared__ __align__(16) uint8_t raw[];
-  Shared& sh = *reinterpret_cast<Shared*>(raw);
+  Shared<kThreads>& sh = *reinterpret_cast<Shared<kThreads>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t r = blockIdx.x / p.pieces;
   const int piece = static_cast<int>(blockIdx.x - r * p.pieces);
@@ -129,167 +266,231 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobP
   const int k = p.k;
 
   // the row's 16-byte vectors: entries [head, head + N * nvec); ragged ends for the first and
-  // last piece
-  const int64_t mis = (reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T);
-  const int64_t head = min(mis == 0 ? (int64_t)0 : N - mis, p.vocab);
-  const int64_t nvec = (p.vocab - head) / N;
-  const int64_t per = ceil_div(nvec, (int64_t)p.pieces);
-  const int64_t vbegin = min(piece * per, nvec), vend = min(vbegin + per, nvec);
+  // last piece. A row has fewer than 2^31 entries.
+  const int vocab = static_cast<int>(p.vocab);
+  const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+  const int head = min(mis == 0 ? 0 : N - mis, vocab);
+  const int nvec = (vocab - head) / N;
+  const int per = ceil_div(nvec, p.pieces);
+  const int vbegin = min(piece * per, nvec), vend = min(vbegin + per, nvec);
   const T* xv = row + head;
 
-  // ---- pass 1
-  const int64_t batches = ceil_div(vend - vbegin, (int64_t)(kThreads * U));  // of every lane
-  const int fold = static_cast<int>(ceil_div(batches, (int64_t)(kMaxima / kThreads)));  // batches an entry covers
-  for (int i = tid; i < kMaxima; i += kThreads) sh.maxima[i] = -INFINITY;
-  if (tid == 0) sh.listed = sh.found = 0;
-  __syncthreads();
-  // a CTA's shared memory may be written to once that CTA runs
-  if (p.pieces > 1) cg::this_cluster().sync();
+  if (tid == 0) sh.listed = sh.found = sh.nan = 0;
   Sums st;
+  st.reset();
+  // ragged ends: fewer than 8 entries each
+  int edge = -1;
+  if (piece == 0 && tid < head) edge = tid;
+  if (piece == p.pieces - 1 && tid >= 32 && head + nvec * N + (tid - 32) < vocab) edge = head + nvec * N + (tid - 32);
+  float edge_x = -INFINITY;
+  if (edge >= 0) {
+    edge_x = elem(row + edge);
+    st.add(edge_x);
+  }
   float lane_max = -INFINITY;
-  int64_t lane_at = -1;  // the first batch that holds lane_max
-  for (int64_t b = 0; b < batches; ++b) {
-    float e[U][N];
-    float bm = -INFINITY;
-    const int64_t v0 = vbegin + b * (kThreads * U) + tid;
+  int lane_at = -1;  // the first batch that holds lane_max
+
+  const int per_batch = kThreads * U;
+  const int whole = (vend - vbegin) / per_batch, batches = ceil_div(vend - vbegin, per_batch);
+  const int fold = max(1, ceil_div(batches, kMaxima / kThreads));  // batches that share an entry of maxima
+  __nv_bfloat16* entry = sh.maxima + tid;
+  int entry_left = fold;
+  float entry_max = -INFINITY;
+  float ref, off, scale;  // of st.m: (x - m) log2 e = t + off
+  auto refer = [&]() {
+    ref = st.m * kLog2eF;
+    off = -fmaf(st.m, kLog2eF, -ref);
+    scale = fabsf(st.m) < kRoom ? exp2_approx(off) : 0.f;
+  };
+  refer();
+  // takes batch b, of which this thread has the vectors e[0 .. valid)
+  auto take = [&](const uint4 (&e)[U], int b, int valid) {
+    float bm = V::max(e[0]);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t v = v0 + u * kThreads;
-      if (v < vend) {
-        unpack16(ldg_nc_v4(xv + v * N), e[u], T());
-      } else {
-#pragma unroll
-        for (int q = 0; q < N; ++q) e[u][q] = -INFINITY;
-      }
+    for (int u = 1; u < U; ++u)
+      if (u < valid) asm("max.NaN.f32 %0, %0, %1;" : "+f"(bm) : "f"(V::max(e[u])));
+    if (!(bm <= st.m + kSlack)) {  // a new reference, or a NaN
+      st.nan |= bm != bm;
+      st.raise(bm);
+      refer();
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int q = 0; q < N; ++q) {
-        bm = fmaxf(bm, e[u][q]);
-        st.nan |= e[u][q] != e[u][q];
-      }
-    st.raise(bm);
-    if (st.m != -INFINITY) {
-      const float m = st.m;
+    if (scale != 0.f) {
       float s = 0.f, w = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int q = 0; q < N; ++q) {
-          const float d = fmaxf(e[u][q] - m, kLowest);  // NaN (inf - inf) too: such rows score NaN
-          const float f = exp2_approx(d * kLog2eF);
-          s += f;
-          w = fmaf(d, f, w);
+      for (int u = 0; u < U; ++u) {
+        if (u < valid) {
+          V::each(V::held(e[u], kLow), [&](float x, int) {
+            const float t = fmaf(x, kLog2eF, -ref);
+            const float f = exp2_approx(t);
+            s += f;
+            w = fmaf(t, f, w);
+          });
         }
-      st.s += s;
-      st.u += w;
+      }
+      w = fmaf(off, s, w) * kLn2;
+      st.s = fmaf(s, scale, st.s);
+      st.u = fmaf(w, scale, st.u);
+    } else if (st.m != -INFINITY) {
+#pragma unroll 1
+      for (int i = 0; i < valid * N; ++i)
+        st.add(elem(xv + (int64_t)(vbegin + b * per_batch + i / N * kThreads + tid) * N + i % N));
     }
     if (k > 0) {
-      float& slot = sh.maxima[(fold == 1 ? (int)b : (int)(b / fold)) * kThreads + tid];
-      slot = fmaxf(slot, bm);
+      entry_max = fmaxf(entry_max, bm);
+      if (--entry_left == 0) {
+        *entry = __float2bfloat16_ru(entry_max);
+        entry += kThreads;
+        entry_left = fold;
+        entry_max = -INFINITY;
+      }
       if (bm > lane_max || lane_at < 0) {
         lane_max = bm;
         lane_at = b;
       }
     }
-  }
-  // ragged ends: fewer than 8 entries each
-  int64_t edge = -1;
-  if (piece == 0 && tid < head) edge = tid;
-  if (piece == p.pieces - 1 && tid >= 32 && head + nvec * N + (tid - 32) < p.vocab) edge = head + nvec * N + (tid - 32);
-  float edge_x = -INFINITY;
-  if (edge >= 0) {
-    edge_x = elem(row + edge);
-    st.nan |= edge_x != edge_x;
-    st.raise(edge_x);
-    if (st.m != -INFINITY) {
-      const float d = fmaxf(edge_x - st.m, kLowest);
-      const float f = exp2_approx(d * kLog2eF);
-      st.s += f;
-      st.u = fmaf(d, f, st.u);
+  };
+  const T* src = xv + (int64_t)(vbegin + tid) * N;
+  const int left = vend - vbegin - whole * per_batch - tid;  // of the last batch, from this thread's first on
+  const int last_valid = whole < batches && left > 0 ? ceil_div(left, kThreads) : 0;
+  auto fetch = [&](int b, int stage) {  // a group of its own, empty past the end
+    if (b < whole) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) copy16(&sh.ring[stage][u][tid], src + u * kThreads * N);
+    } else if (b == whole) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < last_valid) copy16(&sh.ring[stage][u][tid], src + u * kThreads * N);
+    }
+    src += per_batch * N;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(i, i);
+#pragma unroll 1
+  for (int b0 = 0; b0 < whole; b0 += kStages) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+      if (b0 + i < whole) {
+        fetch(b0 + i + kStages - 1, (i + kStages - 1) % kStages);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        uint4 e[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) e[u] = sh.ring[i][u][tid];
+        take(e, b0 + i, U);
+      }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (last_valid > 0) {
+    uint4 e[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) e[u] = sh.ring[whole % kStages][u][tid];
+    take(e, whole, last_valid);
+  }
+  if (k > 0 && (entry_left < fold || last_valid == 0) && entry < sh.maxima + kMaxima)
+    *entry = __float2bfloat16_ru(entry_max);
+  if (k > 0) sh.lane_max[tid] = ordered_bits(fmaxf(lane_max, edge_x) + 0.f);
+  const bool nan_here = st.nan;
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) st.merge(shfl_xor(st, o));
   if (lane == 0) sh.warp[warp] = st;
+  if (nan_here) sh.nan = 1;
+  __syncthreads();  // the ring is free
+  // the pieces' results go to the first CTA once its ring is free too
+  if (p.pieces > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
-  // ---- pass 2: the k largest of the piece
-  int n = 0;
+  // ---- the k largest of the piece
   if (k > 0) {
-    const int entries = static_cast<int>(ceil_div(batches, (int64_t)fold)) * kThreads;
-    // first try: T by value; second: by (value, index)
-    for (int attempt = 0; attempt < 2; ++attempt) {
-      uint64_t mine = make_key(fmaxf(lane_max, edge_x), tid);
-      if (attempt == 1) {  // the best entry of this thread's, with its index
-        mine = 0;
-        if (edge >= 0 && edge_x == edge_x) mine = make_key(edge_x, (uint32_t)edge);
-        if (lane_at >= 0) {
-          for (int u = 0; u < U; ++u) {
-            const int64_t v = vbegin + lane_at * (kThreads * U) + tid + u * kThreads;
+    int n = kCandidates + 1;  // a NaN has no place in the order: the slow way
+    if (!sh.nan) {
+      // first try: the bound by value; second: by (value, index)
+      for (int attempt = 0; attempt < 2; ++attempt) {
+        if (attempt == 0) {
+          if (warp == 0) {
+            const uint32_t t = value_bound<kThreads>(sh.lane_max, k, lane);
+            if (lane == 0) sh.bound = (uint64_t)t << 32;
+          }
+        } else {
+          uint64_t mine = edge >= 0 ? make_key(edge_x, (uint32_t)edge) : 0;  // this thread's best entry
+          for (int u = 0; u < U && lane_at >= 0; ++u) {
+            const int v = vbegin + lane_at * per_batch + u * kThreads + tid;
             for (int q = 0; q < N && v < vend; ++q) {
-              const int64_t idx = head + v * N + q;
-              const float x = elem(row + idx);
-              const uint64_t key = x == x ? make_key(x, (uint32_t)idx) : 0;
+              const uint64_t key = make_key(elem(xv + (int64_t)v * N + q), (uint32_t)(head + v * N + q));
               mine = key > mine ? key : mine;
             }
           }
+          sh.sel.lane_key[tid] = mine;
+          if (tid == 0) sh.listed = sh.found = 0;
+          __syncthreads();
+          int rank = 0;
+          for (int j = 0; j < kThreads; ++j) rank += sh.sel.lane_key[j] > mine || (sh.sel.lane_key[j] == mine && j < tid);
+          if (rank == k - 1) sh.bound = mine;
         }
-        if (tid == 0) sh.listed = sh.found = 0;
+        __syncthreads();
+        const uint64_t bound = sh.bound;
+        const float thr = from_ordered((uint32_t)(bound >> 32));
+        auto collect = [&](float x, int idx) {
+          const uint64_t key = make_key(x, (uint32_t)idx);
+          if (key >= bound) {
+            const int to = atomicAdd(&sh.found, 1);
+            if (to < kCandidates) sh.sel.keys[to] = key;
+          }
+        };
+        if (edge >= 0 && edge_x >= thr) collect(edge_x, edge);
+        if (lane_max >= thr) {
+          for (int i = tid; i < ceil_div(batches, fold) * kThreads; i += kThreads)
+            if (__bfloat162float(sh.maxima[i]) >= thr) sh.sel.list[atomicAdd(&sh.listed, 1)] = (uint16_t)i;
+        }
+        __syncthreads();
+        // a warp reads the U * N entries of a listed batch, four batches in flight
+        const int visits = sh.listed * fold;
+        for (int i0 = warp * 4; i0 < visits; i0 += kWarps * 4) {
+          float x[4];
+          int idx[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            idx[i] = -1;
+            x[i] = 0.f;
+            if (i0 + i < visits && lane < U * N) {
+              const int which = fold == 1 ? i0 + i : (i0 + i) / fold;
+              const int slot = sh.sel.list[which];
+              const int b = slot / kThreads * fold + (fold == 1 ? 0 : i0 + i - which * fold);
+              const int v = vbegin + b * per_batch + (slot % kThreads) + (lane / N) * kThreads;
+              if (v < vend) {
+                idx[i] = head + v * N + lane % N;
+                x[i] = elem(row + idx[i]);
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (idx[i] >= 0 && x[i] >= thr) collect(x[i], idx[i]);
+        }
+        __syncthreads();
+        n = sh.found;
+        if (n <= kCandidates) break;
+        __syncthreads();  // every thread has read `found` before it is cleared
       }
-      sh.lane_key[tid] = mine;
-      __syncthreads();
-      int rank = 0;
-      for (int j = 0; j < kThreads; ++j) rank += sh.lane_key[j] > mine || (sh.lane_key[j] == mine && j < tid);
-      // value alone: any index counts
-      if (rank == k - 1) sh.bound = attempt == 0 ? mine & 0xffffffff00000000ull : mine;
-      __syncthreads();
-      const uint64_t bound = sh.bound;
-      const float thr = from_ordered((uint32_t)(bound >> 32));
-      for (int i = tid; i < entries; i += kThreads)
-        if (bound == 0 || sh.maxima[i] >= thr) sh.list[atomicAdd(&sh.listed, 1)] = i;
-      auto collect = [&](float x, int64_t idx) {
-        if (x == x && make_key(x, (uint32_t)idx) >= bound) {
-          const int at = atomicAdd(&sh.found, 1);
-          if (at < kCandidates) sh.keys[at] = make_key(x, (uint32_t)idx);
-        }
-      };
-      if (edge >= 0) collect(edge_x, edge);
-      __syncthreads();
-      // a warp reads the 32 entries of a listed batch, one a lane
-      for (int i = warp; i < sh.listed; i += kWarps) {
-        const int entry = sh.list[i];
-        const int64_t b0 = (int64_t)(entry / kThreads) * fold;
-        for (int64_t b = b0; b < min(b0 + fold, batches); ++b) {
-          const int64_t v = vbegin + b * (kThreads * U) + (entry % kThreads) + (lane / N) * kThreads;
-          if (v < vend) collect(elem(row + head + v * N + lane % N), head + v * N + lane % N);
-        }
-      }
-      __syncthreads();
-      n = sh.found;
-      if (n <= kCandidates) break;
-      __syncthreads();  // every thread has read `found` before it is cleared
     }
-    uint64_t* best = sh.best[piece];
+    uint64_t* best = sh.sel.best[piece];
     if (n <= kCandidates) {
-      for (int i = tid; i < kMaxK; i += kThreads) best[i] = 0;
-      __syncthreads();
+      for (int i = n + tid; i < k; i += kThreads) best[i] = 0;
       for (int i = tid; i < n; i += kThreads) {
-        const uint64_t mine = sh.keys[i];
+        const uint64_t mine = sh.sel.keys[i];
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += sh.keys[j] > mine;
+        for (int j = 0; j < n; ++j) rank += sh.sel.keys[j] > mine;
         if (rank < k) best[rank] = mine;
       }
     } else {
-      // more entries reach T than the list holds (a few threads own most of the large ones, or
-      // long ties): the next largest key below the last one, k times over the piece
+      // more entries reach T than the list holds (a few threads own most of the large ones), or
+      // a NaN: the next largest key below the last one, k times over the piece
       uint64_t last = ~0ull;
       for (int j = 0; j < k; ++j) {
         if (tid == 0) sh.bound = 0;
         __syncthreads();
         uint64_t top = 0;
-        const int64_t lo = head + vbegin * N, hi = head + vend * N;
-        for (int64_t i = lo + tid; i < hi; i += kThreads) {
+        const int lo = head + vbegin * N, hi = head + vend * N;
+        for (int i = lo + tid; i < hi; i += kThreads) {
           const float x = elem(row + i);
           const uint64_t key = x == x ? make_key(x, (uint32_t)i) : 0;
           if (key < last && key > top) top = key;
@@ -307,27 +508,34 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobP
     }
   }
   __syncthreads();
-  if (tid == 0) {
-    Sums all = sh.warp[0];
-    for (int w = 1; w < kWarps; ++w) all.merge(sh.warp[w]);
-    sh.part[piece] = all;
+  if (warp == 0) {
+    Sums all;
+    all.reset();
+    if (lane < kWarps) all = sh.warp[lane];
+#pragma unroll
+    for (int o = kWarps / 2; o >= 1; o >>= 1) all.merge(shfl_xor(all, o));
+    if (lane == 0) sh.part[piece] = all;
   }
 
   // ---- the pieces meet in the cluster's first CTA
   if (p.pieces > 1) {
     cg::cluster_group cluster = cg::this_cluster();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     __syncthreads();
     if (piece > 0) {
-      Shared* first = cluster.map_shared_rank(&sh, 0);
+      Shared<kThreads>* first = cluster.map_shared_rank(&sh, 0);
       if (tid == 0) first->part[piece] = sh.part[piece];
-      for (int i = tid; i < k; i += kThreads) first->best[piece][i] = sh.best[piece][i];
+      for (int i = tid; i < k; i += kThreads) first->sel.best[piece][i] = sh.sel.best[piece][i];
     }
     cluster.sync();
     if (piece > 0) return;
-    if (tid == 0) {
-      Sums all = sh.part[0];
-      for (int c = 1; c < p.pieces; ++c) all.merge(sh.part[c]);
-      sh.part[0] = all;
+    if (warp == 0) {
+      Sums all;
+      all.reset();
+      if (lane < p.pieces) all = sh.part[lane];
+#pragma unroll
+      for (int o = kMaxCluster / 2; o >= 1; o >>= 1) all.merge(shfl_xor(all, o));
+      if (lane == 0) sh.part[0] = all;
     }
   }
   __syncthreads();
@@ -336,11 +544,11 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobP
   const bool empty = all.m == -INFINITY && !all.nan;
   const float lse = all.nan || all.m == INFINITY ? NAN : (empty ? 0.f : log2f(all.s) * kLn2);
   const float shift = empty ? 0.f : all.m;
-  if (tid == 0) {
+  if (tid == kThreads - 1) {
     const int32_t t = p.targets == nullptr ? -1 : __ldg(p.targets + r);
     float lp = 0.f;
     if (t >= 0) {
-      if (t < p.vocab) {
+      if (t < vocab) {
         lp = (elem(row + t) - shift) - lse;
       } else {
         report(p.err, VFL_DEVERR_SLOT);
@@ -350,14 +558,15 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobP
     p.logprobs[r] = lp;
     p.entropy[r] = empty ? 0.f : lse - all.u / all.s;
   }
-  const int total = p.pieces * kMaxK;
-  for (int i = tid; i < (k > 0 ? total : 0); i += kThreads) {
-    const uint64_t mine = sh.best[i / kMaxK][i % kMaxK];
+  if (k == 0) return;
+  for (int i = tid; i < p.pieces * kMaxK; i += kThreads) {
     if (i % kMaxK >= k) continue;
-    int rank = 0;
-    if (mine != 0) {
+    const uint64_t mine = sh.sel.best[i / kMaxK][i % kMaxK];
+    int rank = i % kMaxK;  // within its piece, whose keys are in order
+    if (p.pieces > 1 && mine != 0) {
+      rank = 0;
       for (int c = 0; c < p.pieces; ++c)
-        for (int j = 0; j < k; ++j) rank += sh.best[c][j] > mine;
+        for (int j = 0; j < k && rank < k; ++j) rank += sh.sel.best[c][j] > mine;
     }
     if (mine != 0 && rank < k) {
       p.values[r * k + rank] = (from_ordered((uint32_t)(mine >> 32)) - shift) - lse;
@@ -365,10 +574,10 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobP
     }
   }
   // entries that are NaN are no alternatives: what is left of the k has none
-  if (k > 0 && all.nan) {
+  if (all.nan) {
     int have = 0;
     for (int c = 0; c < p.pieces; ++c)
-      for (int j = 0; j < k; ++j) have += sh.best[c][j] != 0;
+      for (int j = 0; j < k; ++j) have += sh.sel.best[c][j] != 0;
     for (int j = have + tid; j < k; j += kThreads) {
       p.values[r * k + j] = NAN;
       p.indices[r * k + j] = -1;
@@ -376,23 +585,24 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobP
   }
 }
 
-// CTAs on a row: enough to give every SM one, pieces of at least 8192 entries.
+// CTAs on a row: enough to give every SM one, pieces of at least 4096 entries.
 int choose_pieces(int64_t rows, int64_t vocab) {
   int c = 1;
   while (c < kMaxCluster && rows * c < kNumSMs && vocab / (2 * c) >= 4096) c *= 2;
   return c;
 }
 
-template <typename T>
+template <typename T, int kThreads>
 int launch(const LogprobParams& p, int64_t rows, cudaStream_t stream) {
   static int smem_done[kMaxDevices] = {};
-  auto kern = token_logprobs_kernel<T>;
-  int st = ensure_smem_attribute(reinterpret_cast<const void*>(kern), sizeof(Shared), smem_done);
+  auto kern = token_logprobs_kernel<T, kThreads>;
+  constexpr int kSmem = sizeof(Shared<kThreads>);
+  int st = ensure_smem_attribute(reinterpret_cast<const void*>(kern), kSmem, smem_done);
   if (st) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * p.pieces), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -400,8 +610,15 @@ int launch(const LogprobParams& p, int64_t rows, cudaStream_t stream) {
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.pieces > 1 ? 1 : 0;
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, p), "token_logprobs launch");
+}
+
+// Few CTAs: 512 threads shorten each one's way through its piece. Many: 128, so that an SM holds
+// six or seven rows, whose selections overlap other rows' passes.
+template <typename T>
+int launch_threads(const LogprobParams& p, int64_t rows, cudaStream_t s) {
+  return rows * p.pieces <= 2 * kNumSMs ? launch<T, 512>(p, rows, s) : launch<T, 128>(p, rows, s);
 }
 
 }  // namespace
@@ -419,7 +636,7 @@ extern "C" int vfl_token_logprobs(const void* logits, int32_t dtype, int64_t row
   if (k < 0 || k > kMaxK || k > vocab)
     return fail(VFL_ERR_INVALID_ARGUMENT, "token_logprobs: k %d outside [0, min(%d, vocab)]", k, kMaxK);
   if (rows == 0) return VFL_OK;
-  if (vocab > INT32_MAX || rows > INT32_MAX / kMaxCluster)
+  if (vocab > INT32_MAX - (1 << 20) || rows > INT32_MAX / kMaxCluster)
     return fail(VFL_ERR_UNSUPPORTED, "token_logprobs: %lld x %lld scores", (long long)rows, (long long)vocab);
   if (!logits || !logprobs || !entropy || (k > 0 && (!values || !indices)))
     return fail(VFL_ERR_INVALID_ARGUMENT, "token_logprobs: NULL pointer");
@@ -439,5 +656,5 @@ extern "C" int vfl_token_logprobs(const void* logits, int32_t dtype, int64_t row
   p.values = values;
   p.indices = indices;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == VFL_DTYPE_F32 ? launch<float>(p, rows, s) : launch<__nv_bfloat16>(p, rows, s);
+  return dtype == VFL_DTYPE_F32 ? launch_threads<float>(p, rows, s) : launch_threads<__nv_bfloat16>(p, rows, s);
 }
