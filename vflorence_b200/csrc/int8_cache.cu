@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kMaxWindow = 16;  // rows whose runs one warp stores, at most 31
 
 // Smallest scale kept: the attention divides by V scales, and 2^100 times a context's token
 // count stays inside float32. Blocks whose largest magnitude is below 127 * 2^-100 hold zeros.
@@ -28,10 +29,10 @@ constexpr uint32_t kScaleLocked = 0xffe5a5a5u;
 constexpr uint64_t kLockLimitNs = 500000000ull;
 
 struct AppendParams {
-  const uint8_t* x[2];       // key, value rows
-  int64_t x_stride_bytes[2];
-  int8_t* cache[2];
-  float* scale[2];
+  const uint8_t *key, *value;  // rows
+  int64_t key_stride_bytes, value_stride_bytes;
+  int8_t *k_cache, *v_cache;
+  float *k_scale, *v_scale;
   const int64_t* slots;
   int64_t num_tokens, capacity;
   int num_heads, head_dim, block_size;
@@ -55,6 +56,24 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
   return (uint32_t)(a & 255) | ((uint32_t)(b & 255) << 8) | ((uint32_t)(c & 255) << 16) | ((uint32_t)d << 24);
 }
 
+__device__ __forceinline__ void store_codes(int8_t* dst, const uint32_t (&c)[1]) {
+  __stcg(reinterpret_cast<uint32_t*>(dst), c[0]);
+}
+__device__ __forceinline__ void store_codes(int8_t* dst, const uint32_t (&c)[2]) {
+  __stcg(reinterpret_cast<uint2*>(dst), make_uint2(c[0], c[1]));
+}
+
+// The lock's two sides: what the holder before stored is seen after the first, what this warp
+// stored is seen before the second.
+__device__ __forceinline__ uint32_t exchange_acquire(uint32_t* at, uint32_t v) {
+  uint32_t old;
+  asm volatile("atom.acquire.gpu.global.exch.b32 %0, [%1], %2;" : "=r"(old) : "l"(at), "r"(v) : "memory");
+  return old;
+}
+__device__ __forceinline__ void store_release(uint32_t* at, uint32_t v) {
+  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(at), "r"(v) : "memory");
+}
+
 // code * ratio, rounded, for the four codes of a word.
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   int c[4];
@@ -66,107 +85,150 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   return pack4(c[0], c[1], c[2], c[3]);
 }
 
+// Four codes where every product is within 127 and a rounding error: adding 1.5 * 2^23 rounds it
+// to the whole number in the sum's low bits (to even, as rint does).
+__device__ __forceinline__ uint32_t quantize4(const float* x, float inv) {
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(x[i], inv), 12582912.f));
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+
 // One warp stores the runs that begin in its window of rows, for one head of K or of V. A run is
 // a stretch of consecutive rows whose slots lie in one block: all of an encoder block's tokens,
 // or the one token of a decode step. Its largest magnitude is known before its first code is
-// written, so a block filled by one call is rounded once.
+// written, so a block filled by one call is rounded once. A run of up to kHeld pieces a lane stays
+// in registers from its maximum to its codes; a longer one is read a second time.
 //
 // Two runs of one block in a call (rows of a block that are not neighbours) are taken one after
 // the other: the warp swaps kScaleLocked into the scale before it reads the block and puts the
 // new scale back after its stores. The holder never waits, so the wait ends; it is bounded all
-// the same. The swap is the read of the old scale, so the usual call pays nothing for it.
+// the same. The swap is the read of the old scale, in flight together with the run's own loads.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) append_int8_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads, 3) append_int8_kernel(const AppendParams p) {
   constexpr int kVec = Elem<T>::kVec;
+  constexpr int kHeld = 8;
+  constexpr uint32_t kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
-  const int64_t unit = blockIdx.x * (int64_t)kWarps + (threadIdx.x >> 5);
+  const uint32_t unit = blockIdx.x * (uint32_t)kWarps + (threadIdx.x >> 5);
   // units: (window, K or V, head), heads fastest so that neighbours read neighbouring rows
-  const int per_window = 2 * p.num_heads;
-  const int64_t win = unit / per_window;
-  const int64_t t_begin = win * p.window;
+  const uint32_t win = unit / (2 * p.num_heads);
+  const int64_t t_begin = (int64_t)win * p.window;
   if (t_begin >= p.num_tokens) return;
-  const int rest = static_cast<int>(unit - win * per_window);
-  const int kv = rest / p.num_heads, h = rest - kv * p.num_heads;
-  const int64_t t_end = min(t_begin + p.window, p.num_tokens);
+  const int rest = static_cast<int>(unit - win * (2 * p.num_heads));
+  const bool is_v = rest >= p.num_heads;
+  const int h = is_v ? rest - p.num_heads : rest;
   const int D = p.head_dim, bs = p.block_size;
-  const int vecs = D / kVec;                       // 16-byte pieces of a row
-  const int group = vecs >= 32 ? 32 : next_pow2(vecs);  // lanes on a row
-  const int sub = lane / group, col = lane - sub * group, rows_par = 32 / group;
+  const int vecs = D / kVec;                             // 16-byte pieces of a row
+  const uint32_t inverse = (1u << 20) / vecs + 1;
+  const int64_t stride = is_v ? p.value_stride_bytes : p.key_stride_bytes;
+  const uint8_t* base = (is_v ? p.value : p.key) + (int64_t)h * D * sizeof(T);
+  int8_t* cache = is_v ? p.v_cache : p.k_cache;
+  float* scales = is_v ? p.v_scale : p.k_scale;
 
-  for (int64_t t = t_begin; t < t_end;) {
-    // the row before t decides whether a run begins here
-    const int64_t slot = __ldg(p.slots + t);
-    if (slot < 0 || slot >= p.capacity) {
-      if (slot >= 0 && rest == 0 && lane == 0) report(p.err, VFL_DEVERR_SLOT);
-      ++t;
-      continue;
-    }
-    const int64_t blk = block_of(slot, bs);
-    if (t == t_begin && t > 0) {
-      const int64_t before = __ldg(p.slots + t - 1);
-      if (before >= 0 && before < p.capacity && block_of(before, bs) == blk) {
-        ++t;  // an earlier warp's run
-        while (t < t_end) {
-          const int64_t s = __ldg(p.slots + t);
-          if (s < 0 || s >= p.capacity || block_of(s, bs) != blk) break;
-          ++t;
-        }
-        continue;
+  // the blocks of the window's rows, the row before and those after: lane i has row t_begin - 1 + i
+  auto block_at = [&](int64_t t, int64_t* slot) -> int64_t {
+    *slot = t >= 0 && t < p.num_tokens ? __ldg(p.slots + t) : -1;
+    return *slot >= 0 && *slot < p.capacity ? block_of(*slot, bs) : -1;
+  };
+  int64_t slot;
+  const int64_t blk_l = block_at(t_begin - 1 + lane, &slot);
+  if (rest == 0 && lane >= 1 && lane <= p.window && slot >= p.capacity) report(p.err, VFL_DEVERR_SLOT);
+  const int64_t before = __shfl_up_sync(kAll, blk_l, 1);
+  const uint32_t change = __ballot_sync(kAll, lane >= 1 && blk_l != before);
+  const uint32_t opens = __ballot_sync(kAll, slot >= 0 && blk_l >= 0 && slot == blk_l * bs);  // offset 0
+  uint32_t starts = __ballot_sync(kAll, lane >= 1 && lane <= p.window && blk_l >= 0 && blk_l != before);
+
+  while (starts != 0) {
+    const int at = __ffs(starts) - 1;
+    starts &= starts - 1;
+    const int64_t t = t_begin - 1 + at;
+    const int64_t blk = __shfl_sync(kAll, blk_l, at);
+    const uint32_t after = at < 31 ? change >> (at + 1) << (at + 1) : 0u;  // where the run ends, if it ends here
+    const int stop = after ? __ffs(after) - 1 : 32;
+    int n = stop - at;
+    bool fresh = (opens >> at & (n < 32 ? (1u << n) - 1 : kAll)) != 0;
+    if (!after) {  // past the rows at hand
+      for (;;) {
+        int64_t s;
+        const int64_t b = block_at(t + n + lane, &s);
+        const uint32_t other = __ballot_sync(kAll, b != blk);
+        const int more = other ? __ffs(other) - 1 : 32;
+        fresh |= (__ballot_sync(kAll, lane < more && s == blk * bs)) != 0;
+        n += more;
+        if (other) break;
       }
     }
-    int64_t run_end = t + 1;
-    bool fresh = slot == blk * bs;
-    while (run_end < p.num_tokens) {
-      const int64_t s = __ldg(p.slots + run_end);
-      if (s < 0 || s >= p.capacity || block_of(s, bs) != blk) break;
-      fresh |= s == blk * bs;
-      ++run_end;
-    }
-    const int n = static_cast<int>(run_end - t);
 
+    const int pieces = n * vecs;
+    const int rounds = ceil_div(pieces, kHeld * 32);
+    const bool few = pieces < 4096 && vecs <= 256;  // then (i * inverse) >> 20 = i / vecs
+    uint4 v[kHeld];
+    // a lane's pieces of a round; those past the end read as zeros
+    auto load = [&](int round) {
+#pragma unroll
+      for (int q = 0; q < kHeld; ++q) {
+        const int first = (round * kHeld + q) * 32;
+        v[q] = make_uint4(0u, 0u, 0u, 0u);
+        if (first < pieces) {
+          const int i = first + lane;
+          const int j = few ? (int)((uint32_t)i * inverse >> 20) : i / vecs;
+          if (i < pieces) v[q] = __ldg(reinterpret_cast<const uint4*>(base + (t + j) * stride) + (i - j * vecs));
+        }
+      }
+    };
+    load(0);
     // take the block's scale
-    uint32_t* word = reinterpret_cast<uint32_t*>(p.scale[kv] + blk * p.num_heads + h);
+    uint32_t* word = reinterpret_cast<uint32_t*>(scales + blk * p.num_heads + h);
     uint32_t old_bits = 0;
     if (lane == 0) {
-      old_bits = atomicExch(word, kScaleLocked);
+      old_bits = exchange_acquire(word, kScaleLocked);
       if (old_bits == kScaleLocked) {
         const uint64_t t0 = globaltimer_ns();
         do {
           __nanosleep(100);
-          old_bits = atomicExch(word, kScaleLocked);
+          old_bits = exchange_acquire(word, kScaleLocked);
         } while (old_bits == kScaleLocked && globaltimer_ns() - t0 < kLockLimitNs);
       }
-      __threadfence();
     }
 
     // largest finite magnitude of the run
     float largest = 0.f;
-    bool odd = false;  // an infinity or a NaN
-    const uint8_t* base = p.x[kv] + (int64_t)h * D * sizeof(T);
-    for (int j = sub; j < n; j += rows_par) {
-      const uint4* row = reinterpret_cast<const uint4*>(base + (t + j) * p.x_stride_bytes[kv]);
-      for (int c = col; c < vecs; c += group) {
-        float f[kVec];
-        unpack16(__ldg(row + c), f, T());
+    for (int round = 0;;) {  // a NaN or an infinity stays
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          const float a = fabsf(f[i]);
-          const bool finite = a <= 3.402823466e38f;
-          largest = fmaxf(largest, finite ? a : 0.f);
-          odd |= !finite;
+      for (int q = 0; q < kHeld; ++q) {
+        if ((round * kHeld + q) * 32 < pieces) {
+          float f[kVec];
+          unpack16(v[q], f, T());
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(largest) : "f"(fabsf(f[i])));
+        }
+      }
+      if (++round == rounds) break;
+      load(round);
+    }
+    const bool odd = __any_sync(kAll, !(largest <= 3.402823466e38f));
+    if (odd) {
+      if (lane == 0) report(p.err, VFL_DEVERR_NONFINITE);
+      largest = 0.f;
+      for (int round = 0; round < rounds; ++round) {
+        load(round);
+#pragma unroll
+        for (int q = 0; q < kHeld; ++q) {
+          float f[kVec];
+          unpack16(v[q], f, T());
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) largest = fmaxf(largest, fabsf(f[i]) <= 3.402823466e38f ? fabsf(f[i]) : 0.f);
         }
       }
     }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-    odd = __any_sync(0xffffffffu, odd);
-    old_bits = __shfl_sync(0xffffffffu, old_bits, 0);
+    // magnitudes are ordered as their bits are
+    largest = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(largest)));
+    old_bits = __shfl_sync(kAll, old_bits, 0);
     if (old_bits == kScaleLocked) {  // another run never let go: nothing is stored
       if (lane == 0) report(p.err, VFL_DEVERR_SLOT);
-      t = run_end;
       continue;
     }
-    if (odd && lane == 0) report(p.err, VFL_DEVERR_NONFINITE);
     const float stored = __uint_as_float(old_bits);
     const float old = fresh || !(stored > 0.f) ? 0.f : stored;
     float want = __fmul_rn(largest, 1.f / 127.f);
@@ -174,36 +236,53 @@ __global__ void __launch_bounds__(kThreads) append_int8_kernel(const AppendParam
     const float now = fmaxf(old, want);
     const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
 
-    int8_t* block = p.cache[kv] + (blk * p.num_heads + h) * (int64_t)bs * D;
+    int8_t* block = cache + (blk * p.num_heads + h) * (int64_t)bs * D;
     if (now > old && !fresh) {  // the step grew: the codes the block holds follow
       const float ratio = __fmul_rn(old, inv);
       uint4* b16 = reinterpret_cast<uint4*>(block);
-      for (int i = lane; i < bs * D / 16; i += 32) {
-        uint4 w = __ldcg(b16 + i);
-        w = make_uint4(rescale4(w.x, ratio), rescale4(w.y, ratio), rescale4(w.z, ratio), rescale4(w.w, ratio));
-        __stcg(b16 + i, w);
+      const int words = bs * D / 16;
+      for (int i0 = lane; i0 < words; i0 += 4 * 32) {
+        uint4 w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (i0 + q * 32 < words) w[q] = __ldcg(b16 + i0 + q * 32);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (i0 + q * 32 < words)
+            __stcg(b16 + i0 + q * 32, make_uint4(rescale4(w[q].x, ratio), rescale4(w[q].y, ratio),
+                                                 rescale4(w[q].z, ratio), rescale4(w[q].w, ratio)));
       }
       __syncwarp();  // the new codes overwrite theirs after it
     }
-    for (int j = sub; j < n; j += rows_par) {
-      const int64_t off = __ldg(p.slots + t + j) - blk * bs;
-      const uint4* row = reinterpret_cast<const uint4*>(base + (t + j) * p.x_stride_bytes[kv]);
-      for (int c = col; c < vecs; c += group) {
-        float f[kVec];
-        unpack16(__ldg(row + c), f, T());
-        uint32_t* dst = reinterpret_cast<uint32_t*>(block + off * D + c * kVec);
+    // products past 127 by more than rounding come from infinities and from a tiny scale the cache
+    // held before
+    const bool plain = !odd && __fmul_rn(largest, inv) < 127.5f;
+    for (int round = rounds - 1; round >= 0; --round) {
+      if (round != rounds - 1) load(round);
 #pragma unroll
-        for (int i = 0; i < kVec / 4; ++i)
-          __stcg(dst + i, pack4(quantize(f[4 * i], inv), quantize(f[4 * i + 1], inv), quantize(f[4 * i + 2], inv),
-                                quantize(f[4 * i + 3], inv)));
+      for (int q = 0; q < kHeld; ++q) {
+        const int first = (round * kHeld + q) * 32;
+        if (first < pieces) {
+          const int i = first + lane;
+          const int j = few ? (int)((uint32_t)i * inverse >> 20) : i / vecs;
+          if (i < pieces) {
+            const int64_t off = __ldg(p.slots + t + j) - blk * bs;
+            float f[kVec];
+            unpack16(v[q], f, T());
+            uint32_t c[kVec / 4];
+#pragma unroll
+            for (int e = 0; e < kVec / 4; ++e) {
+              const float* x = f + 4 * e;
+              c[e] = plain ? quantize4(x, inv)
+                           : pack4(quantize(x[0], inv), quantize(x[1], inv), quantize(x[2], inv), quantize(x[3], inv));
+            }
+            store_codes(block + off * D + (i - j * vecs) * kVec, c);
+          }
+        }
       }
     }
     __syncwarp();
-    if (lane == 0) {
-      __threadfence();
-      atomicExch(word, __float_as_uint(now));
-    }
-    t = run_end;
+    if (lane == 0) store_release(word, __float_as_uint(now));
   }
 }
 
@@ -293,26 +372,28 @@ int vfl_reshape_and_cache_int8(const void* key, const void* value, void* k_cache
   AppendParams p;
   st = device_error_word(&p.err);
   if (st) return st;
-  p.x[0] = static_cast<const uint8_t*>(key);
-  p.x[1] = static_cast<const uint8_t*>(value);
-  p.x_stride_bytes[0] = key_token_stride * es;
-  p.x_stride_bytes[1] = value_token_stride * es;
-  p.cache[0] = static_cast<int8_t*>(k_cache);
-  p.cache[1] = static_cast<int8_t*>(v_cache);
-  p.scale[0] = k_scale;
-  p.scale[1] = v_scale;
+  p.key = static_cast<const uint8_t*>(key);
+  p.value = static_cast<const uint8_t*>(value);
+  p.key_stride_bytes = key_token_stride * es;
+  p.value_stride_bytes = value_token_stride * es;
+  p.k_cache = static_cast<int8_t*>(k_cache);
+  p.v_cache = static_cast<int8_t*>(v_cache);
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
   p.slots = slot_mapping;
   p.num_tokens = num_tokens;
   p.capacity = num_blocks * block_size;
   p.num_heads = num_heads;
   p.head_dim = head_dim;
   p.block_size = block_size;
-  // A decode step's rows are runs of one: a window of one row keeps them all in flight. Many
-  // rows are blocks' worth of neighbours: windows of a block leave few warps without a run.
-  p.window = num_tokens * 2 * num_heads <= (int64_t)kNumSMs * 256 ? 1 : (block_size < 64 ? block_size : 64);
+  // A decode step's rows are runs of one: windows of one row keep them all in flight. Many rows
+  // are blocks' worth of neighbours: windows of a block leave few warps without a run.
+  const int most = block_size < kMaxWindow ? block_size : kMaxWindow;
+  const int64_t fit = ceil_div(num_tokens * 2 * num_heads, (int64_t)kNumSMs * 256);
+  p.window = static_cast<int>(fit < most ? fit : most);
   const int64_t warps = ceil_div(num_tokens, (int64_t)p.window) * 2 * num_heads;
   const int64_t ctas = ceil_div(warps, (int64_t)kWarps);
-  if (ctas > INT32_MAX) return fail(VFL_ERR_UNSUPPORTED, "reshape_and_cache_int8: too many tokens");
+  if (warps > INT32_MAX) return fail(VFL_ERR_UNSUPPORTED, "reshape_and_cache_int8: too many tokens");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == VFL_DTYPE_F32)
     append_int8_kernel<float><<<(unsigned)ctas, kThreads, 0, s>>>(p);
