@@ -37,6 +37,7 @@ struct AppendParams {
   int64_t num_tokens, capacity;
   int num_heads, head_dim, block_size;
   int window;                // consecutive rows whose runs one warp takes
+  uint32_t inverse;          // 2^32 / 16-byte pieces of a row, rounded up
   unsigned int* err;
 };
 
@@ -105,9 +106,9 @@ __device__ __forceinline__ uint32_t quantize4(const float* x, float inv) {
 // new scale back after its stores. The holder never waits, so the wait ends; it is bounded all
 // the same. The swap is the read of the old scale, in flight together with the run's own loads.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) append_int8_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads, 4) append_int8_kernel(const AppendParams p) {
   constexpr int kVec = Elem<T>::kVec;
-  constexpr int kHeld = 8;
+  constexpr int kHeld = sizeof(T) == 4 ? 8 : 4;
   constexpr uint32_t kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
   const uint32_t unit = blockIdx.x * (uint32_t)kWarps + (threadIdx.x >> 5);
@@ -120,7 +121,6 @@ __global__ void __launch_bounds__(kThreads, 3) append_int8_kernel(const AppendPa
   const int h = is_v ? rest - p.num_heads : rest;
   const int D = p.head_dim, bs = p.block_size;
   const int vecs = D / kVec;                             // 16-byte pieces of a row
-  const uint32_t inverse = (1u << 20) / vecs + 1;
   const int64_t stride = is_v ? p.value_stride_bytes : p.key_stride_bytes;
   const uint8_t* base = (is_v ? p.value : p.key) + (int64_t)h * D * sizeof(T);
   int8_t* cache = is_v ? p.v_cache : p.k_cache;
@@ -160,24 +160,23 @@ __global__ void __launch_bounds__(kThreads, 3) append_int8_kernel(const AppendPa
       }
     }
 
+    // 16-byte pieces of the run; lane by lane, neighbours in a row first
     const int pieces = n * vecs;
-    const int rounds = ceil_div(pieces, kHeld * 32);
-    const bool few = pieces < 4096 && vecs <= 256;  // then (i * inverse) >> 20 = i / vecs
-    uint4 v[kHeld];
-    // a lane's pieces of a round; those past the end read as zeros
-    auto load = [&](int round) {
-#pragma unroll
-      for (int q = 0; q < kHeld; ++q) {
-        const int first = (round * kHeld + q) * 32;
-        v[q] = make_uint4(0u, 0u, 0u, 0u);
-        if (first < pieces) {
-          const int i = first + lane;
-          const int j = few ? (int)((uint32_t)i * inverse >> 20) : i / vecs;
-          if (i < pieces) v[q] = __ldg(reinterpret_cast<const uint4*>(base + (t + j) * stride) + (i - j * vecs));
-        }
-      }
+    const uint8_t* rows = base + t * stride;
+    auto row_of = [&](int i) -> int {  // i / vecs: the product with the inverse is one too many at most
+      const int j = __umulhi(i, p.inverse);
+      return j - (j * vecs > i);
     };
-    load(0);
+    auto piece = [&](int i) -> uint4 {
+      const int j = row_of(i);
+      return __ldg(reinterpret_cast<const uint4*>(rows + j * stride) + (i - j * vecs));
+    };
+    uint4 v[kHeld];
+#pragma unroll
+    for (int q = 0; q < kHeld; ++q) {
+      v[q] = make_uint4(0u, 0u, 0u, 0u);
+      if (q * 32 + lane < pieces) v[q] = piece(q * 32 + lane);
+    }
     // take the block's scale
     uint32_t* word = reinterpret_cast<uint32_t*>(scales + blk * p.num_heads + h);
     uint32_t old_bits = 0;
@@ -194,32 +193,26 @@ __global__ void __launch_bounds__(kThreads, 3) append_int8_kernel(const AppendPa
 
     // largest finite magnitude of the run
     float largest = 0.f;
-    for (int round = 0;;) {  // a NaN or an infinity stays
+    auto fold = [&](const uint4& w) {  // a NaN stays
+      float f[kVec];
+      unpack16(w, f, T());
 #pragma unroll
-      for (int q = 0; q < kHeld; ++q) {
-        if ((round * kHeld + q) * 32 < pieces) {
-          float f[kVec];
-          unpack16(v[q], f, T());
+      for (int i = 0; i < kVec; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(largest) : "f"(fabsf(f[i])));
+    };
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(largest) : "f"(fabsf(f[i])));
-        }
-      }
-      if (++round == rounds) break;
-      load(round);
-    }
+    for (int q = 0; q < kHeld; ++q) fold(v[q]);
+#pragma unroll 4
+    for (int i = kHeld * 32 + lane; i < pieces; i += 32) fold(piece(i));
     const bool odd = __any_sync(kAll, !(largest <= 3.402823466e38f));
     if (odd) {
       if (lane == 0) report(p.err, VFL_DEVERR_NONFINITE);
       largest = 0.f;
-      for (int round = 0; round < rounds; ++round) {
-        load(round);
+#pragma unroll 1
+      for (int i = lane; i < pieces; i += 32) {
+        float f[kVec];
+        unpack16(piece(i), f, T());
 #pragma unroll
-        for (int q = 0; q < kHeld; ++q) {
-          float f[kVec];
-          unpack16(v[q], f, T());
-#pragma unroll
-          for (int i = 0; i < kVec; ++i) largest = fmaxf(largest, fabsf(f[i]) <= 3.402823466e38f ? fabsf(f[i]) : 0.f);
-        }
+        for (int e = 0; e < kVec; ++e) largest = fmaxf(largest, fabsf(f[e]) <= 3.402823466e38f ? fabsf(f[e]) : 0.f);
       }
     }
     // magnitudes are ordered as their bits are
@@ -254,31 +247,39 @@ __global__ void __launch_bounds__(kThreads, 3) append_int8_kernel(const AppendPa
       }
       __syncwarp();  // the new codes overwrite theirs after it
     }
+    const uint32_t* low = reinterpret_cast<const uint32_t*>(p.slots + t);  // low words of the slots
+    const uint32_t block_low = static_cast<uint32_t>(blk) * static_cast<uint32_t>(bs);
+    auto place = [&](int i) -> int8_t* {
+      const int j = row_of(i);
+      return block + ((__ldg(low + 2 * j) - block_low) * D + (i - j * vecs) * kVec);
+    };
+    auto put = [&](int i, const uint4& w) {
+      float f[kVec];
+      unpack16(w, f, T());
+      uint32_t c[kVec / 4];
+#pragma unroll
+      for (int e = 0; e < kVec / 4; ++e) c[e] = quantize4(f + 4 * e, inv);
+      store_codes(place(i), c);
+    };
     // products past 127 by more than rounding come from infinities and from a tiny scale the cache
     // held before
-    const bool plain = !odd && __fmul_rn(largest, inv) < 127.5f;
-    for (int round = rounds - 1; round >= 0; --round) {
-      if (round != rounds - 1) load(round);
+    if (!odd && __fmul_rn(largest, inv) < 127.5f) {
 #pragma unroll
-      for (int q = 0; q < kHeld; ++q) {
-        const int first = (round * kHeld + q) * 32;
-        if (first < pieces) {
-          const int i = first + lane;
-          const int j = few ? (int)((uint32_t)i * inverse >> 20) : i / vecs;
-          if (i < pieces) {
-            const int64_t off = __ldg(p.slots + t + j) - blk * bs;
-            float f[kVec];
-            unpack16(v[q], f, T());
-            uint32_t c[kVec / 4];
+      for (int q = 0; q < kHeld; ++q)
+        if (q * 32 + lane < pieces) put(q * 32 + lane, v[q]);
+#pragma unroll 4
+      for (int i = kHeld * 32 + lane; i < pieces; i += 32) put(i, piece(i));
+    } else {
+#pragma unroll 1
+      for (int i = lane; i < pieces; i += 32) {
+        float f[kVec];
+        unpack16(piece(i), f, T());
+        uint32_t c[kVec / 4];
 #pragma unroll
-            for (int e = 0; e < kVec / 4; ++e) {
-              const float* x = f + 4 * e;
-              c[e] = plain ? quantize4(x, inv)
-                           : pack4(quantize(x[0], inv), quantize(x[1], inv), quantize(x[2], inv), quantize(x[3], inv));
-            }
-            store_codes(block + off * D + (i - j * vecs) * kVec, c);
-          }
-        }
+        for (int e = 0; e < kVec / 4; ++e)
+          c[e] = pack4(quantize(f[4 * e], inv), quantize(f[4 * e + 1], inv), quantize(f[4 * e + 2], inv),
+                       quantize(f[4 * e + 3], inv));
+        store_codes(place(i), c);
       }
     }
     __syncwarp();
@@ -342,6 +343,8 @@ int check_cache(const char* what, int dtype, int64_t num_tokens, int num_heads, 
   if (num_tokens < 0 || num_heads <= 0 || head_dim <= 0 || block_size <= 0 || num_blocks <= 0)
     return fail(VFL_ERR_INVALID_ARGUMENT, "%s: bad sizes (tokens %lld, heads %d, head_dim %d, block_size %d, blocks %lld)",
                 what, (long long)num_tokens, num_heads, head_dim, block_size, (long long)num_blocks);
+  if ((int64_t)block_size * head_dim > INT32_MAX)
+    return fail(VFL_ERR_UNSUPPORTED, "%s: block_size %d times head_dim %d", what, block_size, head_dim);
   if (head_dim % 16 != 0)
     return fail(VFL_ERR_UNSUPPORTED, "%s: head_dim %d must be a multiple of 16", what, head_dim);
   return VFL_OK;
@@ -386,6 +389,7 @@ int vfl_reshape_and_cache_int8(const void* key, const void* value, void* k_cache
   p.num_heads = num_heads;
   p.head_dim = head_dim;
   p.block_size = block_size;
+  p.inverse = UINT32_MAX / static_cast<uint32_t>(head_dim * es / 16) + 1;
   // A decode step's rows are runs of one: windows of one row keep them all in flight. Many rows
   // are blocks' worth of neighbours: windows of a block leave few warps without a run.
   const int most = block_size < kMaxWindow ? block_size : kMaxWindow;
