@@ -10,11 +10,11 @@
 // forbidden token) adds nothing. Bound: HBM, the row read once.
 //
 // One pass gives the sums and, in shared memory, the largest value of each thread's batches of four
-// 16-byte vectors. A value T is then taken that at least k, and not many more, of the threads' own
-// maxima reach: a lower bound of the k-th largest entry, since the maxima are distinct entries.
+// 16-byte vectors. A value T is then taken that at least k, and not many more, of the maxima of 128 groups
+// of threads reach: a lower bound of the k-th largest entry, since the maxima are distinct entries.
 // Only batches whose maximum reaches T, a few more than k, are read again, from L2; their entries
 // >= T are ranked by counting. (A bound from the first batches, with entries picked up as they
-// pass, reads nothing twice but collects six times as many: 58 us against 35 at 1024 x 51289,
+// pass, reads nothing twice but collects six times as many: 58 us against 36 at 1024 x 51289,
 // k = 20.) Where ties at T overflow the list (rows of mostly one value), the bound becomes the k-th
 // best (value, index) pair of the threads' best entries and the collection runs again. A row is
 // cut over a cluster of up to 8 CTAs when there are few rows; the pieces meet in the first CTA's
@@ -22,6 +22,9 @@
 //
 // The pass is close to two other bounds: 1024 x 51289 bfloat16 entries are 11.5 a clock and SM at
 // the copy rate, the exponentials allow 16, and at about 6 instructions an entry the issue rate 21.
+// Measured there: 24 us without alternatives (4.4 TB/s), 35 with k = 20, whose selection all rows
+// reach at the same time; 4 x 50265 float32: 4.6 and (k = 5) 8.1 us, where the selection's short
+// steps, each run once, are most of the time.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -36,6 +39,7 @@ namespace {
 constexpr int kMaxK = 64;
 constexpr int kStages = 3;          // batches of a thread in flight
 constexpr int kCandidates = 1024;
+constexpr int kGroups = 128;        // of threads, whose maxima bound the k-th largest entry
 constexpr int kMaxCluster = 8;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2eF = 1.4426950408889634f;
@@ -91,14 +95,6 @@ struct Sums {
       s += f;
       u = fmaf(d, f, u);
     }
-  }
-  __device__ __forceinline__ void merge(Sums o) {
-    nan |= o.nan;
-    const float top = fmaxf(m, o.m);
-    raise(top);
-    o.raise(top);
-    s += o.s;
-    u += o.u;
   }
 };
 
@@ -162,13 +158,16 @@ struct Vec<__nv_bfloat16> {
   }
 };
 
-__device__ __forceinline__ Sums shfl_xor(const Sums& a, int mask) {
-  Sums o;
-  o.m = __shfl_xor_sync(0xffffffffu, a.m, mask);
-  o.s = __shfl_xor_sync(0xffffffffu, a.s, mask);
-  o.u = __shfl_xor_sync(0xffffffffu, a.u, mask);
-  o.nan = __shfl_xor_sync(0xffffffffu, (int)a.nan, mask) != 0;
-  return o;
+// The sums of a warp's lanes, against the largest of their maxima, in every lane.
+__device__ __forceinline__ void merge_warp(Sums& a) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  a.nan = __any_sync(kAll, a.nan);
+  a.raise(from_ordered(__reduce_max_sync(kAll, ordered_bits(a.m))));
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    a.s += __shfl_xor_sync(kAll, a.s, o);
+    a.u += __shfl_xor_sync(kAll, a.u, o);
+  }
 }
 
 struct LogprobParams {
@@ -207,7 +206,7 @@ struct Shared {
   };
   // of the threads' batches, rounded up to 16 bits; longer pieces fold batches together
   __nv_bfloat16 maxima[Selection<kThreads>::kMaxima];
-  uint32_t lane_max[kThreads];
+  uint32_t group_max[kGroups];
   Sums part[kMaxCluster];
   Sums warp[kThreads / 32];
   int listed, found, nan;
@@ -218,16 +217,16 @@ __device__ __forceinline__ void copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
-// A value that at least k of the threads' maxima reach, and where ties allow not many more: found
-// by halving, in one warp.
-template <int kThreads>
+// A value that at least k of the groups' maxima reach, and where ties allow not many more: found by
+// halving, in one warp (counting each maximum's rank by a thread of its own is no faster in one CTA
+// and 5 us slower with seven on an SM).
 __device__ __forceinline__ uint32_t value_bound(const uint32_t* maxima, int k, int lane) {
-  uint32_t v[kThreads / 32];
+  uint32_t v[kGroups / 32];
 #pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) v[i] = maxima[i * 32 + lane];
+  for (int i = 0; i < kGroups / 32; ++i) v[i] = maxima[i * 32 + lane];
   uint32_t lo = v[0], hi = v[0];
 #pragma unroll
-  for (int i = 1; i < kThreads / 32; ++i) {
+  for (int i = 1; i < kGroups / 32; ++i) {
     lo = min(lo, v[i]);
     hi = max(hi, v[i]);
   }
@@ -238,8 +237,7 @@ __device__ __forceinline__ uint32_t value_bound(const uint32_t* maxima, int k, i
     const uint32_t mid = lo + (hi - lo + 1) / 2;
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) c += v[i] >= mid;
-    c = __reduce_add_sync(0xffffffffu, c);
+    for (int i = 0; i < kGroups / 32; ++i) c += __popc(__ballot_sync(0xffffffffu, v[i] >= mid));
     if (c >= k) {
       lo = mid;
       if (c <= k + k / 2 + 4) break;
@@ -276,6 +274,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
   const T* xv = row + head;
 
   if (tid == 0) sh.listed = sh.found = sh.nan = 0;
+  // the target's entry, in flight while the row passes: at the end the two loads cost 1 to 2 us
+  int32_t target = -1;
+  float target_x = NAN;
+  if (tid == kThreads - 1 && piece == 0 && p.targets != nullptr) {
+    target = __ldg(p.targets + r);
+    if (target >= 0 && target < vocab) target_x = elem(row + target);
+  }
   Sums st;
   st.reset();
   // ragged ends: fewer than 8 entries each
@@ -389,10 +394,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
   }
   if (k > 0 && (entry_left < fold || last_valid == 0) && entry < sh.maxima + kMaxima)
     *entry = __float2bfloat16_ru(entry_max);
-  if (k > 0) sh.lane_max[tid] = ordered_bits(fmaxf(lane_max, edge_x) + 0.f);
-  const bool nan_here = st.nan;
+  if (k > 0) {
+    uint32_t top = ordered_bits(fmaxf(lane_max, edge_x) + 0.f);
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) st.merge(shfl_xor(st, o));
+    for (int o = 1; o < kThreads / kGroups; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    sh.group_max[tid / (kThreads / kGroups)] = top;
+  }
+  const bool nan_here = st.nan;
+  merge_warp(st);
   if (lane == 0) sh.warp[warp] = st;
   if (nan_here) sh.nan = 1;
   __syncthreads();  // the ring is free
@@ -407,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
       for (int attempt = 0; attempt < 2; ++attempt) {
         if (attempt == 0) {
           if (warp == 0) {
-            const uint32_t t = value_bound<kThreads>(sh.lane_max, k, lane);
+            const uint32_t t = value_bound(sh.group_max, k, lane);
             if (lane == 0) sh.bound = (uint64_t)t << 32;
           }
         } else {
@@ -438,32 +447,37 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
         };
         if (edge >= 0 && edge_x >= thr) collect(edge_x, edge);
         if (lane_max >= thr) {
-          for (int i = tid; i < ceil_div(batches, fold) * kThreads; i += kThreads)
-            if (__bfloat162float(sh.maxima[i]) >= thr) sh.sel.list[atomicAdd(&sh.listed, 1)] = (uint16_t)i;
+          constexpr int kMine = kMaxima / kThreads;
+          const int mine = ceil_div(batches, fold);
+          uint32_t mask = 0;
+#pragma unroll
+          for (int i = 0; i < kMine; ++i)
+            if (i < mine && __bfloat162float(sh.maxima[i * kThreads + tid]) >= thr) mask |= 1u << i;
+          int to = atomicAdd(&sh.listed, __popc(mask));
+          for (; mask != 0; mask &= mask - 1) sh.sel.list[to++] = (uint16_t)((__ffs(mask) - 1) * kThreads + tid);
         }
         __syncthreads();
-        // a warp reads the U * N entries of a listed batch, four batches in flight
+        // a warp reads the U * N entries of a listed batch, eight batches in flight; lanes without
+        // an entry read one that is there and drop it, so that no branch parts the loads
+        constexpr int kFlight = 8;
         const int visits = sh.listed * fold;
-        for (int i0 = warp * 4; i0 < visits; i0 += kWarps * 4) {
-          float x[4];
-          int idx[4];
+        for (int i0 = warp; i0 < visits; i0 += kWarps * kFlight) {
+          float x[kFlight];
+          int idx[kFlight];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            idx[i] = -1;
-            x[i] = 0.f;
-            if (i0 + i < visits && lane < U * N) {
-              const int which = fold == 1 ? i0 + i : (i0 + i) / fold;
-              const int slot = sh.sel.list[which];
-              const int b = slot / kThreads * fold + (fold == 1 ? 0 : i0 + i - which * fold);
-              const int v = vbegin + b * per_batch + (slot % kThreads) + (lane / N) * kThreads;
-              if (v < vend) {
-                idx[i] = head + v * N + lane % N;
-                x[i] = elem(row + idx[i]);
-              }
-            }
+          for (int i = 0; i < kFlight; ++i) {
+            const int visit = min(i0 + i * kWarps, visits - 1);
+            const int which = fold == 1 ? visit : visit / fold;
+            const int slot = sh.sel.list[which];
+            const int b = slot / kThreads * fold + (visit - which * fold);
+            const int v = vbegin + b * per_batch + (slot % kThreads) + (lane / N) * kThreads;
+            const bool there = i0 + i * kWarps < visits && lane < U * N && v < vend;
+            const int at = head + (there ? v : vbegin) * N + lane % N;
+            x[i] = elem(row + at);
+            idx[i] = there ? at : -1;
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < kFlight; ++i)
             if (idx[i] >= 0 && x[i] >= thr) collect(x[i], idx[i]);
         }
         __syncthreads();
@@ -512,8 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
     Sums all;
     all.reset();
     if (lane < kWarps) all = sh.warp[lane];
-#pragma unroll
-    for (int o = kWarps / 2; o >= 1; o >>= 1) all.merge(shfl_xor(all, o));
+    merge_warp(all);
     if (lane == 0) sh.part[piece] = all;
   }
 
@@ -533,8 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
       Sums all;
       all.reset();
       if (lane < p.pieces) all = sh.part[lane];
-#pragma unroll
-      for (int o = kMaxCluster / 2; o >= 1; o >>= 1) all.merge(shfl_xor(all, o));
+      merge_warp(all);
       if (lane == 0) sh.part[0] = all;
     }
   }
@@ -545,32 +557,26 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) token_logprobs_kern
   const float lse = all.nan || all.m == INFINITY ? NAN : (empty ? 0.f : log2f(all.s) * kLn2);
   const float shift = empty ? 0.f : all.m;
   if (tid == kThreads - 1) {
-    const int32_t t = p.targets == nullptr ? -1 : __ldg(p.targets + r);
-    float lp = 0.f;
-    if (t >= 0) {
-      if (t < vocab) {
-        lp = (elem(row + t) - shift) - lse;
-      } else {
-        report(p.err, VFL_DEVERR_SLOT);
-        lp = NAN;
-      }
-    }
-    p.logprobs[r] = lp;
+    if (target >= vocab) report(p.err, VFL_DEVERR_SLOT);
+    p.logprobs[r] = target >= 0 ? (target_x - shift) - lse : 0.f;
     p.entropy[r] = empty ? 0.f : lse - all.u / all.s;
   }
   if (k == 0) return;
-  for (int i = tid; i < p.pieces * kMaxK; i += kThreads) {
-    if (i % kMaxK >= k) continue;
-    const uint64_t mine = sh.sel.best[i / kMaxK][i % kMaxK];
-    int rank = i % kMaxK;  // within its piece, whose keys are in order
-    if (p.pieces > 1 && mine != 0) {
-      rank = 0;
+  auto put = [&](uint64_t key, int rank) {
+    p.values[r * k + rank] = (from_ordered((uint32_t)(key >> 32)) - shift) - lse;
+    p.indices[r * k + rank] = (int32_t)~(uint32_t)key;
+  };
+  if (p.pieces == 1) {
+    if (tid < k && sh.sel.best[0][tid] != 0) put(sh.sel.best[0][tid], tid);
+  } else {
+    for (int i = tid; i < p.pieces * kMaxK; i += kThreads) {
+      const uint64_t mine = i % kMaxK < k ? sh.sel.best[i / kMaxK][i % kMaxK] : 0;
+      if (mine == 0) continue;
+      int rank = 0;
       for (int c = 0; c < p.pieces; ++c)
-        for (int j = 0; j < k && rank < k; ++j) rank += sh.sel.best[c][j] > mine;
-    }
-    if (mine != 0 && rank < k) {
-      p.values[r * k + rank] = (from_ordered((uint32_t)(mine >> 32)) - shift) - lse;
-      p.indices[r * k + rank] = (int32_t)~(uint32_t)mine;
+#pragma unroll 4
+        for (int j = 0; j < k; ++j) rank += sh.sel.best[c][j] > mine;
+      if (rank < k) put(mine, rank);
     }
   }
   // entries that are NaN are no alternatives: what is left of the k has none
