@@ -314,18 +314,19 @@ struct Query {
           v[0] = v[1] = v[2] = v[3] = 0.f;
           if (on) load4(src + k_dim<D>(w, ln.tq), v);
         }
-        int c[4];
+        // adding 1.5 * 2^23 leaves the whole number in the sum's mantissa. Its digits base 256 in
+        // [-128, 127]: with 128 added to each they are the bytes of a plain number, and a byte
+        // loses the 128 again by flipping its top bit
+        constexpr uint32_t kBias = S::kPlanes == 3 ? 0x808080u : 0x8080u;
+        uint32_t c[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = __float2int_rn(v[i] * to_int);
+        for (int i = 0; i < 4; ++i)
+          c[i] = (__float_as_uint(fmaf(v[i], to_int, 12582912.f)) - 0x4b400000u + kBias) ^ kBias;
 #pragma unroll
-        for (int plane = S::kPlanes - 1; plane >= 0; --plane) {
-          // digits base 256 in [-128, 127], the lowest first
-          uint32_t packed = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            packed |= (uint32_t)(c[i] & 255) << (8 * i);
-            c[i] = (c[i] - (int)(int8_t)c[i]) >> 8;
-          }
+        for (int plane = 0; plane < S::kPlanes; ++plane) {
+          constexpr uint32_t kPick[3] = {0x0040, 0x0051, 0x0062};  // byte 0, 1, 2 of two words
+          const uint32_t pick = kPick[S::kPlanes - 1 - plane];
+          const uint32_t packed = __byte_perm(__byte_perm(c[0], c[1], pick), __byte_perm(c[2], c[3], pick), 0x5410);
           const int at = (nt * S::kPlanes + plane) * S::kWords + w;
           if (S::kQueryInSmem) {
             q_smem[at * 32 + ln.lane] = packed;
@@ -833,6 +834,10 @@ void choose_shape(vfl_attention_int8_plan* plan, int64_t items, int64_t tiles_su
     const int64_t by_len = ceil_div(longest, (int64_t)2 * plan->warps);
     splits = splits < by_len ? splits : by_len;
     if (longest <= 512 && splits > kMaxCluster) splits = kMaxCluster;
+    // clusters do not fill every GPC (with two CTAs an SM 71 of 4 and 33 of 8 were measured to fit):
+    // one more is a second wave (72 float32 items of 16 rows: 20 us over clusters of 4, 17 of 2)
+    if (splits >= 8 && splits < 16 && 100 * items > 89 * (slots / 8)) splits = 4;
+    if (splits >= 4 && splits < 8 && 100 * items > 96 * (slots / 4)) splits = 2;
   }
   set_splits(plan, splits);
 }
