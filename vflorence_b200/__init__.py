@@ -3,7 +3,8 @@
 Modules
     paged_ops      the vllm_cpu_attn functions (get_isa, get_scheduler_metadata,
                    reshape_and_cache, attention_with_kv_cache) + copy_blocks, prepare_decode,
-                   paged_slots - thin Python over the C ABI in include/vflorence_b200.h
+                   paged_slots, the 8-bit cache and its attention, 4-bit linear layers, token
+                   scores - thin Python over the C ABI in include/vflorence_b200.h
     attention      the vflorence::self_attention / vflorence::cross_attention custom ops and
                    stage_cross (imported on demand: importing it registers the ops)
     context        the per-step Context the ops read

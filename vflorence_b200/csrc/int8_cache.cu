@@ -110,7 +110,7 @@ __device__ __forceinline__ uint32_t quantize4(const float* x, float inv) {
 // kEven: a row's pieces divide the warp, so a lane's pieces are a fixed step of rows apart (32 x 572
 // tokens of 12 x 128 bfloat16: 49 us, by a multiplication a piece 61).
 //
-// Measured: 64 x 585 tokens of 12 x 64 bfloat16 62 us, 172 MB at 2.8 TB/s: about 700 instructions a
+// Measured: 64 x 585 tokens of 12 x 64 bfloat16 62 us, 172 MB at 2.8 TB/s: about 630 instructions a
 // run of 16 rows at 0.55 a clock and scheduler are the bound, and the registers (64, for four CTAs an
 // SM) what keeps them from more. 256 single tokens 8.6 us, a few 3.7 us: the chain of slot, scale
 // and block.

@@ -1,5 +1,6 @@
 """The four ``vllm_cpu_attn`` functions the vflorence engine calls, on B200, plus the two ops
-that sit beside them (copy-on-write block copies and the per-step metadata build).
+that sit beside them (copy-on-write block copies and the per-step metadata build) and the
+operators of a decode step in fewer bits.
 
 Drop-in use: ``import vflorence_b200.paged_ops as vllm_cpu_attn``. Signatures and argument
 meaning follow the call sites in vflorence (paths inside that project):
@@ -11,6 +12,16 @@ meaning follow the call sites in vflorence (paths inside that project):
     copy_blocks               replaces ModelRunner._copy_blocks, model_runner.py:162-167
     prepare_decode            replaces the list building of ModelRunner._prepare, :290-306
     paged_slots               replaces the encoder slot arithmetic of _encode, :240-242
+
+A decode step in fewer bits, and the scores that show what the fewer bits cost (no counterpart
+in vflorence):
+
+    reshape_and_cache_int8        the append into an 8-bit cache, a scale for each block and head
+    gather_kv_int8                its tokens back in full precision
+    get_scheduler_metadata_int8   the plan of the attention over it
+    attention_with_kv_cache_int8  attention over it; grouped heads, causal rows, beams
+    quantize_int4, linear_int4    linear layers with 4-bit weights and group scales
+    token_logprobs                log probabilities of given tokens, entropy, likeliest alternatives
 
 Differences a caller sees:
   * caches, queries, keys, values and outputs live on one CUDA device; a CPU one is an error
