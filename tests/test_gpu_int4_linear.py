@@ -65,6 +65,22 @@ def test_linear_k_ends_inside_a_chunk_and_long_k(dtype, group, k):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("group,k", [(32, 4224), (64, 4224), (32, 4192), (128, 4224), (256, 4352), (32, 10368)])
+def test_linear_reads_nothing_past_its_operands(dtype, group, k):
+    """A long k is cut over several CTAs, whose last one has less: what lies behind the scales, the
+    codes and x is not read (a NaN would meet zeros there and stay)."""
+    x, codes, scales, bias = make(3, 40, k, group, dtype, seed=k)
+
+    def walled(t, wall):
+        room = torch.full((t.numel() + 4096,), wall, dtype=t.dtype, device="cuda")
+        room[: t.numel()] = t.flatten().cuda()
+        return room[: t.numel()].view(t.shape)
+
+    got = ops.linear_int4(walled(x, math.nan), walled(codes, 255), walled(scales, math.nan), walled(bias, math.nan))
+    check(got, x, codes, scales, bias, False)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_linear_strides_and_out(dtype):
     x, codes, scales, bias = make(4, 48, 256, 64, dtype)
     wide = torch.zeros((4, 320), dtype=dtype, device="cuda")

@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) int4_linear_kernel(
           pc[i] += kChunk / 2;
         }
         if (kBlocks > 1 && wide_scales) {
-          load_scales<kBlocks * sizeof(T)>(ps + f_group, scale[stage]);
+          load_scales<kBlocks * sizeof(T)>(ps + min(f_group, groups - kBlocks), scale[stage]);  // past k: the last ones
         } else {
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b) scale[stage][b] = __ldg(ps + min(f_group + b, groups - 1));
