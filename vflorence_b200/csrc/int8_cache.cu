@@ -110,14 +110,17 @@ __device__ __forceinline__ uint32_t quantize4(const float* x, float inv) {
 // kEven: a row's pieces divide the warp, so a lane's pieces are a fixed step of rows apart (32 x 572
 // tokens of 12 x 128 bfloat16: 49 us, by a multiplication a piece 61).
 //
+// kOneRow (windows of one row, as in a decode step): a lane holds one piece and eight CTAs share an
+// SM, spills and all, since the chain of slot, scale and block is the time: 256 single tokens of
+// 16 x 64 6.4 us, 512 of 16 x 128 10.8 us; by the other variant 8.7 and 15.1, by six CTAs 7.7 and 11.8.
+//
 // Measured: 64 x 585 tokens of 12 x 64 bfloat16 62 us, 172 MB at 2.8 TB/s: about 630 instructions a
-// run of 16 rows at 0.55 a clock and scheduler are the bound, and the registers (64, for four CTAs an
-// SM) what keeps them from more. 256 single tokens 8.6 us, a few 3.7 us: the chain of slot, scale
-// and block.
-template <typename T, bool kEven>
-__global__ void __launch_bounds__(kThreads, 4) append_int8_kernel(const AppendParams p) {
+// run of 16 rows at 0.54 a clock and scheduler are the bound, and the registers (64, for four CTAs an
+// SM) what keeps them from more. A few tokens take 3.4 us.
+template <typename T, bool kEven, bool kOneRow>
+__global__ void __launch_bounds__(kThreads, kOneRow ? 8 : 4) append_int8_kernel(const AppendParams p) {
   constexpr int kVec = Elem<T>::kVec;
-  constexpr int kHeld = sizeof(T) == 4 ? 8 : 4;
+  constexpr int kHeld = kOneRow ? 1 : (sizeof(T) == 4 ? 8 : 4);
   constexpr uint32_t kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
   const uint32_t unit = blockIdx.x * (uint32_t)kWarps + (threadIdx.x >> 5);
@@ -447,11 +450,13 @@ int vfl_reshape_and_cache_int8(const void* key, const void* value, void* k_cache
   if (warps > INT32_MAX) return fail(VFL_ERR_UNSUPPORTED, "reshape_and_cache_int8: too many tokens");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool even = 32 % row_pieces == 0;
-  if (dtype == VFL_DTYPE_F32)
-    (even ? append_int8_kernel<float, true> : append_int8_kernel<float, false>)<<<(unsigned)ctas, kThreads, 0, s>>>(p);
-  else
-    (even ? append_int8_kernel<__nv_bfloat16, true>
-          : append_int8_kernel<__nv_bfloat16, false>)<<<(unsigned)ctas, kThreads, 0, s>>>(p);
+  auto pick = [&](auto type) {
+    using T = decltype(type);
+    if (p.window == 1) return even ? append_int8_kernel<T, true, true> : append_int8_kernel<T, false, true>;
+    return even ? append_int8_kernel<T, true, false> : append_int8_kernel<T, false, false>;
+  };
+  auto kern = dtype == VFL_DTYPE_F32 ? pick(float()) : pick(__nv_bfloat16());
+  kern<<<(unsigned)ctas, kThreads, 0, s>>>(p);
   return cuda_status(cudaGetLastError(), "reshape_and_cache_int8 launch");
 }
 
