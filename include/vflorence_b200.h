@@ -363,14 +363,16 @@ int vfl_fork_token_rows(int32_t* tokens, int64_t row_stride, int32_t num_rows, i
  * hold anything.
  *
  * vfl_reshape_and_cache_int8 stores the tokens of key / value (as vfl_reshape_and_cache) at
- * their slots, in 8 bits. For each run of consecutive tokens in one block, and each head, with a
- * the largest finite magnitude of the run:
- *     s' = max(s, a * (1/127)), s = the block's scale, 0 when the run writes offset 0 (the block
+ * their slots, in 8 bits. For each block that the call writes, and each head, with a the largest
+ * finite magnitude of the call's tokens in the block:
+ *     s' = max(s, a * (1/127)), s = the block's scale, 0 when the call writes offset 0 (the block
  *          starts anew) or when it is not above 0; a * (1/127) below 2^-100 counts as 0;
  *     codes the block holds become rint(code * (s * (1/s'))) when s' > s and it did not start anew;
  *     new codes are rint(x * (1/s')) held to [-127, 127], 0 when s' is 0.
- * Infinities are held to +-127 and NaNs to 0, flagged VFL_DEVERR_NONFINITE. Tokens of one block
- * that are not neighbours in the call are stored one run after the other, in no set order.
+ * Infinities are held to +-127 and NaNs to 0, flagged VFL_DEVERR_NONFINITE. The order of the tokens
+ * changes nothing (but two tokens of one slot, of which either is kept); a block's tokens that are
+ * not neighbours in the call take several times longer. Calls that write the same block are to be
+ * ordered (one stream, or events).
  * head_dim a multiple of 16; pointers and token strides 16-byte aligned. */
 int vfl_reshape_and_cache_int8(const void* key, const void* value, void* k_cache, void* v_cache,
                                float* k_scale, float* v_scale, const int64_t* slot_mapping,

@@ -2,11 +2,12 @@
 //
 // A block's tokens of one head share a float32 scale: codes int8 [num_blocks, H, block_size, D],
 // scales [num_blocks, H], value = code * scale. The append keeps a block consistent while it
-// fills: with a = the largest finite magnitude of the new tokens, s' = max(s, a * (1/127)); when
-// s' > s the codes the block holds are brought to the new step, rint(code * (s * (1/s'))), and
-// the new ones are rint(x * (1/s')) held to [-127, 127]. Writing offset 0 starts a block anew
-// (s = 0). Products in float32 with one rounding each, so that a plain restatement gives the
-// same codes bit for bit. A growth rounds the older codes once more (at most half a step).
+// fills: with a = the largest finite magnitude of the call's tokens in the block, s' = max(s, a *
+// (1/127)); when s' > s the codes the block holds are brought to the new step, rint(code * (s *
+// (1/s'))), and the new ones are rint(x * (1/s')) held to [-127, 127]. A call that writes offset 0
+// starts the block anew (s = 0). Products in float32 with one rounding each, so that a plain
+// restatement gives the same codes bit for bit. A growth rounds the older codes once more (at most
+// half a step).
 //
 // Both kernels move bytes: the bound is HBM for many tokens and one dependent round trip (slot,
 // then the block's scale and the token) for a few.
@@ -17,16 +18,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kCtas = 4;        // of many rows, that an SM is to hold
 constexpr int kMaxWindow = 16;  // rows whose runs one warp stores, at most 31
 
 // Smallest scale kept: the attention divides by V scales, and 2^100 times a context's token
 // count stays inside float32. Blocks whose largest magnitude is below 127 * 2^-100 hold zeros.
 constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100
-
-// The value a scale has while a run of tokens of its block is being stored: a NaN payload that
-// no arithmetic makes. It doubles as the block's lock, see append_int8_kernel.
-constexpr uint32_t kScaleLocked = 0xffe5a5a5u;
-constexpr uint64_t kLockLimitNs = 500000000ull;
 
 struct AppendParams {
   const uint8_t *key, *value;  // rows
@@ -39,6 +36,7 @@ struct AppendParams {
   int window;                // consecutive rows whose runs one warp takes
   uint32_t inverse;          // 2^32 / 16-byte pieces of a row, rounded up
   int rows_per_warp;         // 32 / pieces of a row
+  uint32_t parts;            // CTAs that share a window's heads
   unsigned int* err;
 };
 
@@ -65,17 +63,6 @@ __device__ __forceinline__ void store_codes(int8_t* dst, const uint32_t (&c)[2])
   __stcg(reinterpret_cast<uint2*>(dst), make_uint2(c[0], c[1]));
 }
 
-// The lock's two sides: what the holder before stored is seen after the first, what this warp
-// stored is seen before the second.
-__device__ __forceinline__ uint32_t exchange_acquire(uint32_t* at, uint32_t v) {
-  uint32_t old;
-  asm volatile("atom.acquire.gpu.global.exch.b32 %0, [%1], %2;" : "=r"(old) : "l"(at), "r"(v) : "memory");
-  return old;
-}
-__device__ __forceinline__ void store_release(uint32_t* at, uint32_t v) {
-  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(at), "r"(v) : "memory");
-}
-
 // code * ratio, rounded, for the four codes of a word.
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   int c[4];
@@ -96,226 +83,502 @@ __device__ __forceinline__ uint32_t quantize4(const float* x, float inv) {
   return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
 
-// One warp stores the runs that begin in its window of rows, for one head of K or of V. A run is
-// a stretch of consecutive rows whose slots lie in one block: all of an encoder block's tokens,
-// or the one token of a decode step. Its largest magnitude is known before its first code is
-// written, so a block filled by one call is rounded once. A run of up to kHeld pieces a lane stays
-// in registers from its maximum to its codes; a longer one is read a second time.
-//
-// Two runs of one block in a call (rows of a block that are not neighbours) are taken one after
-// the other: the warp swaps kScaleLocked into the scale before it reads the block and puts the
-// new scale back after its stores. The holder never waits, so the wait ends; it is bounded all
-// the same. The swap is the read of the old scale, in flight together with the run's own loads.
-//
-// kEven: a row's pieces divide the warp, so a lane's pieces are a fixed step of rows apart (32 x 572
-// tokens of 12 x 128 bfloat16: 49 us, by a multiplication a piece 61).
-//
-// kOneRow (windows of one row, as in a decode step): a lane holds one piece and eight CTAs share an
-// SM, spills and all, since the chain of slot, scale and block is the time: 256 single tokens of
-// 16 x 64 6.4 us, 512 of 16 x 128 10.8 us; by the other variant 8.7 and 15.1, by six CTAs 7.7 and 11.8.
-//
-// Measured: 64 x 585 tokens of 12 x 64 bfloat16 62 us, 172 MB at 2.8 TB/s: about 630 instructions a
-// run of 16 rows at 0.54 a clock and scheduler are the bound, and the registers (64, for four CTAs an
-// SM) what keeps them from more. A few tokens take 3.4 us.
-template <typename T, bool kEven, bool kOneRow>
-__global__ void __launch_bounds__(kThreads, kOneRow ? 8 : 4) append_int8_kernel(const AppendParams p) {
+constexpr float kFloatMax = 3.402823466e38f;
+
+// The scale of a block that held tokens of step `old` and takes tokens of magnitude `largest`.
+__device__ __forceinline__ float next_scale(float old, float largest) {
+  const float want = __fmul_rn(largest, 1.f / 127.f);
+  return fmaxf(old, want < kMinScale ? 0.f : want);
+}
+
+// Codes of `bytes` bytes of a block, brought to another step by one warp.
+__device__ __forceinline__ void rescale_block(int8_t* block, int bytes, float ratio, int lane) {
+  uint4* b16 = reinterpret_cast<uint4*>(block);
+  const int words = bytes / 16;
+  for (int i0 = lane; i0 < words; i0 += 4 * 32) {
+    uint4 w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (i0 + q * 32 < words) w[q] = __ldcg(b16 + i0 + q * 32);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (i0 + q * 32 < words)
+        __stcg(b16 + i0 + q * 32, make_uint4(rescale4(w[q].x, ratio), rescale4(w[q].y, ratio),
+                                             rescale4(w[q].z, ratio), rescale4(w[q].w, ratio)));
+  }
+  __syncwarp();  // the new codes overwrite theirs after it
+}
+
+// Low words of the slots of rows r0 + lane, r0 + 32 + lane ...
+template <int kLook>
+__device__ __forceinline__ void look_at(const AppendParams& p, int r0, uint32_t (&word)[kLook]) {
+  const uint32_t* low = reinterpret_cast<const uint32_t*>(p.slots + r0 + (threadIdx.x & 31));
+  if (r0 + 32 * kLook <= p.num_tokens) {
+#pragma unroll
+    for (int u = 0; u < kLook; ++u) word[u] = __ldg(low + u * 64);
+  } else {
+    const int left = p.num_tokens - r0 - static_cast<int>(threadIdx.x & 31);
+#pragma unroll
+    for (int u = 0; u < kLook; ++u) word[u] = u * 32 < left ? __ldg(low + u * 64) : 0xffffffffu;
+  }
+}
+
+// Whether one of these rows may lie in the `bs` slots from slot0 on (or among slots 2^32 apart)
+template <int kLook>
+__device__ __forceinline__ bool may_hit(const uint32_t (&word)[kLook], int64_t slot0, int bs) {
+  uint32_t least = 0xffffffffu;
+#pragma unroll
+  for (int u = 0; u < kLook; ++u) least = __viaddmin_u32(word[u], 0u - (uint32_t)slot0, least);
+  return least < (uint32_t)bs;
+}
+
+// The run that begins at row t, and where `more_rows` says so the later rows of its block, stored by
+// a warp piece by piece: blocks whose rows are not neighbours, infinities and NaNs among the tokens, and
+// products past 127 by more than rounding (from a tiny scale the cache held before).
+template <typename T>
+__device__ __noinline__ void store_slowly(const AppendParams& p, bool is_v, int h, int blk, int t, bool more_rows) {
   constexpr int kVec = Elem<T>::kVec;
-  constexpr int kHeld = kOneRow ? 1 : (sizeof(T) == 4 ? 8 : 4);
   constexpr uint32_t kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
-  const uint32_t unit = blockIdx.x * (uint32_t)kWarps + (threadIdx.x >> 5);
-  // units: (window, K or V, head), heads fastest so that neighbours read neighbouring rows
-  const uint32_t win = unit / (2 * p.num_heads);
-  const int t_begin = win * p.window;
-  if (t_begin >= p.num_tokens) return;
-  const int rest = static_cast<int>(unit - win * (2 * p.num_heads));
-  const bool is_v = rest >= p.num_heads;
-  const int h = is_v ? rest - p.num_heads : rest;
-  const int D = p.head_dim, bs = p.block_size;
-  const int vecs = D / kVec;                             // 16-byte pieces of a row
-  const int stride = is_v ? p.value_stride_bytes : p.key_stride_bytes;
+  const int D = p.head_dim, bs = p.block_size, vecs = D / kVec;
+  const int64_t slot0 = (int64_t)blk * bs, at_head = (int64_t)blk * p.num_heads + h;
   const uint8_t* base = (is_v ? p.value : p.key) + (int64_t)h * D * sizeof(T);
-  int8_t* cache = is_v ? p.v_cache : p.k_cache;
-  float* scales = is_v ? p.v_scale : p.k_scale;
-
-  // the blocks of the window's rows, the row before and those after: lane i has row t_begin - 1 + i
-  // (-1: no slot, -2: a slot past the pool)
-  auto block_at = [&](int t, bool* opens) -> int {
-    const int64_t slot = t >= 0 && t < p.num_tokens ? __ldg(p.slots + t) : -1;
-    *opens = false;
-    if (slot < 0) return -1;
-    if (slot >= p.capacity) return -2;
-    const int blk = static_cast<int>(block_of(slot, bs));
-    *opens = slot == (int64_t)blk * bs;  // offset 0
-    return blk;
+  const int stride = is_v ? p.value_stride_bytes : p.key_stride_bytes;
+  int8_t* block = (is_v ? p.v_cache : p.k_cache) + at_head * (bs * D);
+  float* scale_at = (is_v ? p.v_scale : p.k_scale) + at_head;
+  auto each = [&](auto&& take) {
+    constexpr int kLook = 16;
+    unsigned long long had = 0;  // offsets met: up to 64 slots they tell when the block is complete
+    bool done = false;
+#pragma unroll 1
+    for (int r0 = t; r0 < p.num_tokens && !done; r0 += 32 * kLook) {
+      uint32_t word[kLook];
+      look_at(p, r0, word);
+      if (!__any_sync(kAll, may_hit(word, slot0, bs))) continue;
+#pragma unroll 1
+      for (int j0 = r0; j0 < min(r0 + 32 * kLook, p.num_tokens) && !done; j0 += 32) {
+        const int64_t slot = j0 + lane < p.num_tokens ? __ldg(p.slots + j0 + lane) : -1;
+        uint32_t rows = __ballot_sync(kAll, (uint64_t)(slot - slot0) < (uint64_t)bs);
+        if (!more_rows) {
+          done = rows != kAll;
+          rows &= ~(rows + 1);  // those before the first of another block
+        }
+#pragma unroll 1
+        for (; rows != 0; rows &= rows - 1) {
+          const int l = __ffs(rows) - 1;
+          const uint32_t offset = __shfl_sync(kAll, (uint32_t)(slot - slot0), l);
+          had |= 1ull << (offset & 63);
+          const uint4* row = reinterpret_cast<const uint4*>(base + (j0 + l) * (int64_t)stride);
+#pragma unroll 1
+          for (int c = lane; c < vecs; c += 32) take(__ldg(row + c), offset, c);
+        }
+        done |= bs <= 64 && __popcll(had) == bs;
+      }
+    }
   };
+  float largest = 0.f;
+  bool odd = false, zero = false;
+  each([&](const uint4& w, uint32_t offset, int) {
+    float f[kVec];
+    unpack16(w, f, T());
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const bool finite = fabsf(f[e]) <= kFloatMax;
+      largest = fmaxf(largest, finite ? fabsf(f[e]) : 0.f);
+      odd |= !finite;
+    }
+    zero |= offset == 0;
+  });
+  if (odd) report(p.err, VFL_DEVERR_NONFINITE);
+  largest = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(largest)));
+  const bool fresh = __any_sync(kAll, zero);
+  const float stored = __ldcg(scale_at);
+  const float old = fresh || !(stored > 0.f) ? 0.f : stored;
+  const float now = next_scale(old, largest);
+  const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
+  if (now > old && !fresh) rescale_block(block, bs * D, __fmul_rn(old, inv), lane);
+  each([&](const uint4& w, uint32_t offset, int c) {
+    float f[kVec];
+    unpack16(w, f, T());
+    uint32_t codes[kVec / 4];
+#pragma unroll
+    for (int e = 0; e < kVec / 4; ++e)
+      codes[e] = pack4(quantize(f[4 * e], inv), quantize(f[4 * e + 1], inv), quantize(f[4 * e + 2], inv),
+                       quantize(f[4 * e + 3], inv));
+    store_codes(block + (offset * D + c * kVec), codes);
+  });
+  __syncwarp();  // every lane has read the old scale
+  if (lane == 0) *scale_at = now;
+}
+
+// What a warp works on: one head of K or of V. The CTAs of a window share its heads; a last warp may
+// have none (`on` is false): it takes part in what its CTA does.
+struct Side {
+  const uint8_t* base;  // the head's rows
+  int stride;
+  int8_t* cache;
+  float* scales;
+  int h;
+  bool on, is_v;
+  __device__ __forceinline__ Side(const AppendParams& p, int elem_size) {
+    const int rest = static_cast<int>(blockIdx.x % p.parts * (blockDim.x >> 5) + (threadIdx.x >> 5));
+    on = rest < 2 * p.num_heads;
+    is_v = on && rest >= p.num_heads;
+    h = !on ? 0 : (is_v ? rest - p.num_heads : rest);
+    base = (is_v ? p.value : p.key) + (int64_t)h * p.head_dim * elem_size;
+    stride = is_v ? p.value_stride_bytes : p.key_stride_bytes;
+    cache = is_v ? p.v_cache : p.k_cache;
+    scales = is_v ? p.v_scale : p.k_scale;
+  }
+};
+
+// Row t's block (-1: no slot, -2: a slot past the pool), whether it is the block's first slot, and the
+// slot less the row, which is the same all along a run in order.
+__device__ __forceinline__ int block_at(const AppendParams& p, int t, bool* opens, uint32_t* lead) {
+  const int64_t slot = t >= 0 && t < p.num_tokens ? __ldg(p.slots + t) : -1;
+  *opens = false;
+  *lead = (uint32_t)slot - t;
+  if (slot < 0) return -1;
+  if (slot >= p.capacity) return -2;
+  const int blk = static_cast<int>(block_of(slot, p.block_size));
+  *opens = slot == (int64_t)blk * p.block_size;
+  return blk;
+}
+
+// Goes on with a run of block `blk` from its n-th row on, past the rows that a warp has at hand.
+__device__ __forceinline__ void extend_run(const AppendParams& p, int t, int blk, uint32_t lead, int* n, bool* open,
+                                           bool* in_order) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  for (;;) {
+    bool open_b;
+    uint32_t lead_b;
+    const int b = block_at(p, t + *n + lane, &open_b, &lead_b);
+    const uint32_t other = __ballot_sync(kAll, b != blk);
+    const int more = other ? __ffs(other) - 1 : 32;
+    *open |= __any_sync(kAll, lane < more && open_b);
+    *in_order &= !__any_sync(kAll, lane < more && lead_b != lead);
+    *n += more;
+    if (other) return;
+  }
+}
+
+// The 16-byte pieces of a run, neighbours in a row first.
+template <typename T>
+struct Pieces {
+  const uint8_t* rows;
+  int stride, vecs, count;
+  uint32_t inverse;
+  __device__ __forceinline__ Pieces(const AppendParams& p, const Side& side, int t, int n)
+      : rows(side.base + t * (int64_t)side.stride), stride(side.stride), vecs(p.head_dim / Elem<T>::kVec),
+        count(n * vecs), inverse(p.inverse) {}
+  // row of piece i, and its place in it: the product with the inverse is one too many at most
+  __device__ __forceinline__ int row(int i, int* c) const {
+    int j = __umulhi(i, inverse);
+    j -= j * vecs > i;
+    *c = i - j * vecs;
+    return j;
+  }
+  __device__ __forceinline__ uint4 load(int j, int c) const {
+    return __ldg(reinterpret_cast<const uint4*>(rows + j * (int64_t)stride) + c);
+  }
+};
+
+// largest = the larger of it and the magnitudes of a piece; a NaN stays
+template <typename T>
+__device__ __forceinline__ void fold(float& largest, const uint4& w) {
+  float f[Elem<T>::kVec];
+  unpack16(w, f, T());
+#pragma unroll
+  for (int i = 0; i < Elem<T>::kVec; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(largest) : "f"(fabsf(f[i])));
+}
+
+template <typename T>
+__device__ __forceinline__ void put(int8_t* to, const uint4& w, float inv) {
+  constexpr int kVec = Elem<T>::kVec;
+  float f[kVec];
+  unpack16(w, f, T());
+  uint32_t codes[kVec / 4];
+#pragma unroll
+  for (int e = 0; e < kVec / 4; ++e) codes[e] = quantize4(f + 4 * e, inv);
+  store_codes(to, codes);
+}
+
+// A warp stores a run of consecutive rows in one block: all of an encoder block's tokens, or the one
+// token of a decode step. Its largest magnitude is known before its first code is written, so a block
+// filled by one call is rounded once.
+//
+// A block may have other rows in the call (time-major prompts; a padding row in a block's middle). Its
+// first run stores them all: every run that is not a whole block in order (which leaves no slot to
+// another row) has its CTA look through the slots of the call. So a block is written by one warp a head
+// and needs no lock, and the order of the rows changes nothing.
+
+// The runs of many rows: a warp takes those that begin in its window of rows. A run of up to kHeld pieces
+// a lane stays in registers from its maximum to its codes; a longer one is read a second time.
+//
+// kEven: a row's pieces divide the warp, so a lane's pieces are a fixed step of rows apart.
+//
+// Measured: 64 x 585 tokens of 12 x 64 bfloat16 64 us, 172 MB at 2.7 TB/s: the instructions of a run (some
+// 600 for 16 rows) at about half a clock and scheduler are the bound, and the registers (64, for four CTAs
+// an SM; three with 80: 59, but 2000 single tokens of 16 x 64 48 instead of 45) what keeps them from more.
+// 64 x 576 without a partly filled block 59. The same 64 x 585 rows token by token of all requests, which
+// take the slow way block by block: 1.0 ms.
+template <typename T, bool kEven>
+__global__ void __launch_bounds__(kThreads, kCtas) append_int8_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int kVec = Elem<T>::kVec;
+  constexpr int kHeld = 4;
+  constexpr uint32_t kAll = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  const int t_begin = blockIdx.x / p.parts * p.window;
+  const Side side(p, sizeof(T));
+  const int D = p.head_dim, bs = p.block_size;
+
+  // lane i has row t_begin - 1 + i: those of the window, the one before and those after
   bool open_l;
-  const int blk_l = block_at(t_begin - 1 + lane, &open_l);
-  if (rest == 0 && lane >= 1 && lane <= p.window && blk_l == -2) report(p.err, VFL_DEVERR_SLOT);
+  uint32_t lead_l;
+  const int blk_l = block_at(p, t_begin - 1 + lane, &open_l, &lead_l);
+  if (side.on && side.h == 0 && !side.is_v && lane >= 1 && lane <= p.window && blk_l == -2) report(p.err, VFL_DEVERR_SLOT);
   const int before = __shfl_up_sync(kAll, blk_l, 1);
   const uint32_t change = __ballot_sync(kAll, lane >= 1 && blk_l != before);
   const uint32_t opens = __ballot_sync(kAll, open_l);
   uint32_t starts = __ballot_sync(kAll, lane >= 1 && lane <= p.window && blk_l >= 0 && blk_l != before);
 
-  while (starts != 0) {
-    const int at = __ffs(starts) - 1;
-    starts &= starts - 1;
-    const int t = t_begin - 1 + at;
+  // the runs' lengths (lane i: of the run at row t_begin - 1 + i), whether they write offset 0, and
+  // which of them are not a whole block in order
+  int n_l = 0;
+  uint32_t fresh = 0, partial = 0;
+#pragma unroll 1
+  for (uint32_t left = starts; left != 0; left &= left - 1) {
+    const int at = __ffs(left) - 1;
     const int blk = __shfl_sync(kAll, blk_l, at);
+    const uint32_t lead = __shfl_sync(kAll, lead_l, at);
     const uint32_t after = at < 31 ? change >> (at + 1) << (at + 1) : 0u;  // where the run ends, if it ends here
-    const int stop = after ? __ffs(after) - 1 : 32;
-    int n = stop - at;
-    bool fresh = (opens >> at & (n < 32 ? (1u << n) - 1 : kAll)) != 0;
-    if (!after) {  // past the rows at hand
-      for (;;) {
-        bool open;
-        const int b = block_at(t + n + lane, &open);
-        const uint32_t other = __ballot_sync(kAll, b != blk);
-        const int more = other ? __ffs(other) - 1 : 32;
-        fresh |= (__ballot_sync(kAll, lane < more && open)) != 0;
-        n += more;
-        if (other) break;
+    int n = (after ? __ffs(after) - 1 : 32) - at;
+    const uint32_t here = (n < 32 ? (1u << n) - 1 : kAll) << at;
+    bool open = (opens & here) != 0;
+    bool in_order = (__ballot_sync(kAll, lead_l != lead) & here) == 0;
+    if (!after && !(in_order && n == bs)) extend_run(p, t_begin - 1 + at, blk, lead, &n, &open, &in_order);
+    if (lane == at) n_l = n;
+    fresh |= open ? 1u << at : 0u;
+    partial |= in_order && n == bs ? 0u : 1u << at;
+  }
+
+  // other rows of these runs' blocks (bit i: of the run's at row t_begin - 1 + i), looked for by the CTA
+  uint32_t apart = 0;
+  if (partial != 0) {
+    constexpr int kLook = 16;
+    uint32_t hits = 0, earlier = 0;
+    // the warp's i-th chunk of rows: chunks go from the window's down to the first, then up
+    const int chunks = ceil_div(p.num_tokens, 32 * kLook), at_window = t_begin / (32 * kLook);
+    auto look = [&](int i) {
+      const int r0 = (i <= at_window ? at_window - i : i) * (32 * kLook);
+      uint32_t word[kLook];
+      look_at(p, r0, word);
+#pragma unroll 1
+      for (uint32_t left = partial; left != 0; left &= left - 1) {
+        const int at = __ffs(left) - 1;
+        const int t = t_begin - 1 + at, n = __shfl_sync(kAll, n_l, at);
+        const int64_t slot0 = (int64_t)__shfl_sync(kAll, blk_l, at) * bs;
+        if (__any_sync(kAll, may_hit(word, slot0, bs))) {  // the whole slots decide
+#pragma unroll 1
+          for (int row = r0 + lane; row < min(r0 + 32 * kLook, p.num_tokens); row += 32) {
+            if ((uint64_t)(__ldg(p.slots + row) - slot0) >= (uint64_t)bs || (uint32_t)(row - t) < (uint32_t)n) continue;
+            hits |= 1u << at;
+            earlier |= row < t ? 1u << at : 0u;
+          }
+          __syncwarp();
+        }
+      }
+    };
+    __shared__ uint32_t s_hits, s_earlier;
+    auto gather = [&]() {  // the CTA's bits, in every thread
+      if (!__syncthreads_or(hits != 0)) return;
+      if (threadIdx.x == 0) s_hits = s_earlier = 0;
+      __syncthreads();
+      atomicOr(&s_hits, hits);
+      atomicOr(&s_earlier, earlier);
+      __syncthreads();
+      hits = s_hits;
+      earlier = s_earlier;
+      __syncthreads();
+    };
+    const int warps = blockDim.x >> 5;
+    int i = threadIdx.x >> 5;
+    if (i < chunks) look(i);
+    if (chunks > warps) {  // rows of a block apart are near, most often: then this was enough for all but the first
+      gather();
+      if ((earlier & partial) != partial) {
+#pragma unroll 1
+        for (i += warps; i < chunks; i += warps) look(i);
       }
     }
+    gather();
+    starts &= ~earlier;  // a block's first run stores all its rows
+    apart = hits & ~earlier;
+  }
+  if (!side.on) return;
 
-    // 16-byte pieces of the run; lane by lane, neighbours in a row first
-    const int pieces = n * vecs;
-    const uint8_t* rows = base + t * (int64_t)stride;
-    auto row_of = [&](int i) -> int {  // i / vecs: the product with the inverse is one too many at most
-      const int j = __umulhi(i, p.inverse);
-      return j - (j * vecs > i);
-    };
-    const int j0 = row_of(lane), c0 = lane - j0 * vecs;
+  uint32_t slow = apart;  // runs left for the end
+  for (starts &= ~apart; starts != 0; starts &= starts - 1) {
+    const int at = __ffs(starts) - 1;
+    const int t = t_begin - 1 + at;
+    const int blk = __shfl_sync(kAll, blk_l, at), n = __shfl_sync(kAll, n_l, at);
+    const float stored = __ldcg(side.scales + (int64_t)blk * p.num_heads + side.h);
+    const Pieces<T> run(p, side, t, n);
+    int c0;
+    const int j0 = run.row(lane, &c0);
     // row and place in it of this lane's piece i = lane + 32 q
     auto find = [&](int i, int* c) -> int {
-      if (kEven) {
-        *c = c0;
-        return j0 + (i >> 5) * p.rows_per_warp;
-      }
-      const int j = row_of(i);
-      *c = i - j * vecs;
-      return j;
+      if (!kEven) return run.row(i, c);
+      *c = c0;
+      return j0 + (i >> 5) * p.rows_per_warp;
     };
     auto piece = [&](int i) -> uint4 {
       int c;
       const int j = find(i, &c);
-      return __ldg(reinterpret_cast<const uint4*>(rows + j * (int64_t)stride) + c);
+      return run.load(j, c);
     };
     uint4 v[kHeld];
 #pragma unroll
     for (int q = 0; q < kHeld; ++q) {
       v[q] = make_uint4(0u, 0u, 0u, 0u);
-      if (q * 32 + lane < pieces) v[q] = piece(q * 32 + lane);
+      if (q * 32 + lane < run.count) v[q] = piece(q * 32 + lane);
     }
-    // take the block's scale
-    uint32_t* word = reinterpret_cast<uint32_t*>(scales + (int64_t)blk * p.num_heads + h);
-    uint32_t old_bits = 0;
-    if (lane == 0) {
-      old_bits = exchange_acquire(word, kScaleLocked);
-      if (old_bits == kScaleLocked) {
-        const uint64_t t0 = globaltimer_ns();
-        do {
-          __nanosleep(100);
-          old_bits = exchange_acquire(word, kScaleLocked);
-        } while (old_bits == kScaleLocked && globaltimer_ns() - t0 < kLockLimitNs);
-      }
+    float largest = 0.f;  // finite magnitude of the run
+#pragma unroll
+    for (int q = 0; q < kHeld; ++q) {
+      if (q * 32 >= run.count) break;
+      fold<T>(largest, v[q]);
     }
-
-    // largest finite magnitude of the run
-    float largest = 0.f;
-    auto fold = [&](const uint4& w) {  // a NaN stays
-      float f[kVec];
-      unpack16(w, f, T());
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(largest) : "f"(fabsf(f[i])));
-    };
-#pragma unroll
-    for (int q = 0; q < kHeld; ++q) fold(v[q]);
 #pragma unroll 4
-    for (int i = kHeld * 32 + lane; i < pieces; i += 32) fold(piece(i));
-    const bool odd = __any_sync(kAll, !(largest <= 3.402823466e38f));
-    if (odd) {
-      if (lane == 0) report(p.err, VFL_DEVERR_NONFINITE);
-      largest = 0.f;
-#pragma unroll 1
-      for (int i = lane; i < pieces; i += 32) {
-        float f[kVec];
-        unpack16(piece(i), f, T());
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) largest = fmaxf(largest, fabsf(f[e]) <= 3.402823466e38f ? fabsf(f[e]) : 0.f);
-      }
-    }
+    for (int i = kHeld * 32 + lane; i < run.count; i += 32) fold<T>(largest, piece(i));
+    const bool odd = __any_sync(kAll, !(largest <= kFloatMax));
     // magnitudes are ordered as their bits are
     largest = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(largest)));
-    old_bits = __shfl_sync(kAll, old_bits, 0);
-    if (old_bits == kScaleLocked) {  // another run never let go: nothing is stored
-      if (lane == 0) report(p.err, VFL_DEVERR_SLOT);
+    const bool anew = fresh >> at & 1;
+    const float old = anew || !(stored > 0.f) ? 0.f : stored;
+    const float now = next_scale(old, largest);
+    const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
+    int8_t* block = side.cache + ((int64_t)blk * p.num_heads + side.h) * (bs * D);
+    if (odd || !(__fmul_rn(largest, inv) < 127.5f)) {
+      slow |= 1u << at;
       continue;
     }
-    const float stored = __uint_as_float(old_bits);
-    const float old = fresh || !(stored > 0.f) ? 0.f : stored;
-    float want = __fmul_rn(largest, 1.f / 127.f);
-    want = want < kMinScale ? 0.f : want;
-    const float now = fmaxf(old, want);
-    const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
-
-    int8_t* block = cache + ((int64_t)blk * p.num_heads + h) * (bs * D);
-    if (now > old && !fresh) {  // the step grew: the codes the block holds follow
-      const float ratio = __fmul_rn(old, inv);
-      uint4* b16 = reinterpret_cast<uint4*>(block);
-      const int words = bs * D / 16;
-      for (int i0 = lane; i0 < words; i0 += 4 * 32) {
-        uint4 w[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (i0 + q * 32 < words) w[q] = __ldcg(b16 + i0 + q * 32);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (i0 + q * 32 < words)
-            __stcg(b16 + i0 + q * 32, make_uint4(rescale4(w[q].x, ratio), rescale4(w[q].y, ratio),
-                                                 rescale4(w[q].z, ratio), rescale4(w[q].w, ratio)));
-      }
-      __syncwarp();  // the new codes overwrite theirs after it
-    }
+    if (now > old && !anew) rescale_block(block, bs * D, __fmul_rn(old, inv), lane);  // the step grew
     const uint32_t* low = reinterpret_cast<const uint32_t*>(p.slots + t);  // low words of the slots
-    const uint32_t block_low = static_cast<uint32_t>(blk) * static_cast<uint32_t>(bs);
     auto place = [&](int i) -> int8_t* {
       int c;
       const int j = find(i, &c);
-      return block + ((__ldg(low + 2 * j) - block_low) * D + c * kVec);
+      return block + ((__ldg(low + 2 * j) - (uint32_t)blk * (uint32_t)bs) * D + c * kVec);
     };
-    auto put = [&](int i, const uint4& w) {
-      float f[kVec];
-      unpack16(w, f, T());
-      uint32_t c[kVec / 4];
 #pragma unroll
-      for (int e = 0; e < kVec / 4; ++e) c[e] = quantize4(f + 4 * e, inv);
-      store_codes(place(i), c);
-    };
-    // products past 127 by more than rounding come from infinities and from a tiny scale the cache
-    // held before
-    if (!odd && __fmul_rn(largest, inv) < 127.5f) {
-#pragma unroll
-      for (int q = 0; q < kHeld; ++q)
-        if (q * 32 + lane < pieces) put(q * 32 + lane, v[q]);
-#pragma unroll 4
-      for (int i = kHeld * 32 + lane; i < pieces; i += 32) put(i, piece(i));
-    } else {
-#pragma unroll 1
-      for (int i = lane; i < pieces; i += 32) {
-        float f[kVec];
-        unpack16(piece(i), f, T());
-        uint32_t c[kVec / 4];
-#pragma unroll
-        for (int e = 0; e < kVec / 4; ++e)
-          c[e] = pack4(quantize(f[4 * e], inv), quantize(f[4 * e + 1], inv), quantize(f[4 * e + 2], inv),
-                       quantize(f[4 * e + 3], inv));
-        store_codes(place(i), c);
-      }
+    for (int q = 0; q < kHeld; ++q) {
+      if (q * 32 >= run.count) break;
+      if (q * 32 + lane < run.count) put<T>(place(q * 32 + lane), v[q], inv);
     }
-    __syncwarp();
-    if (lane == 0) store_release(word, __float_as_uint(now));
+#pragma unroll 4
+    for (int i = kHeld * 32 + lane; i < run.count; i += 32) put<T>(place(i), piece(i), inv);
+    if (lane == 0) side.scales[(int64_t)blk * p.num_heads + side.h] = now;
   }
+#pragma unroll 1
+  for (; slow != 0; slow &= slow - 1) {
+    const int at = __ffs(slow) - 1;
+    store_slowly<T>(p, side.is_v, side.h, __shfl_sync(kAll, blk_l, at), t_begin - 1 + at, apart >> at & 1);
+  }
+}
+
+// Few rows, as in a decode step: a CTA has one row, whose run is most often itself, and eight CTAs share
+// an SM. The chain of slot, token and store is the time, so the slots of the other rows are read with
+// the row's own. 4 tokens of 16 x 64 float32 3.0 us, 256 of bfloat16 6.2, 512 of 16 x 128 10.3.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 8) append_int8_row_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int kVec = Elem<T>::kVec;
+  constexpr int kLook = 4;
+  constexpr uint32_t kAll = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  const int t = blockIdx.x / p.parts, bs = p.block_size;
+  uint32_t word[kLook];
+  const int warp_rows = (blockDim.x >> 5) * (32 * kLook);
+  int r0 = (threadIdx.x >> 5) * (32 * kLook);
+  if (r0 < p.num_tokens) look_at(p, r0, word);
+  bool open_l;
+  uint32_t lead_l;
+  const int blk_l = block_at(p, t - 1 + lane, &open_l, &lead_l);
+  const int blk = __shfl_sync(kAll, blk_l, 1);
+  if (blk == -2 && blockIdx.x % p.parts == 0 && threadIdx.x == 0) report(p.err, VFL_DEVERR_SLOT);
+  if (blk < 0 || blk == __shfl_sync(kAll, blk_l, 0)) return;
+  const Side side(p, sizeof(T));
+  const uint32_t lead = __shfl_sync(kAll, lead_l, 1);
+  const uint32_t after = __ballot_sync(kAll, blk_l != blk) >> 1;
+  int n = after ? __ffs(after) - 1 : 31;
+  const uint32_t here = ((1u << n) - 1) << 1;
+  bool anew = (__ballot_sync(kAll, open_l) & here) != 0;
+  bool in_order = (__ballot_sync(kAll, lead_l != lead) & here) == 0;
+  if (!after) extend_run(p, t, blk, lead, &n, &anew, &in_order);
+
+  const Pieces<T> run(p, side, t, n);
+  float* const scale_at = side.scales + (int64_t)blk * p.num_heads + side.h;
+  const float stored = __ldcg(scale_at);
+  int c0;
+  const int j0 = run.row(lane, &c0);
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (lane < run.count) v = run.load(j0, c0);
+
+  bool apart = false;
+  if (!(in_order && n == bs)) {
+    const int64_t slot0 = (int64_t)blk * bs;
+    bool hit = false, earlier = false;
+#pragma unroll 1
+    while (r0 < p.num_tokens) {
+      if (__any_sync(kAll, may_hit(word, slot0, bs))) {  // the whole slots decide
+#pragma unroll 1
+        for (int row = r0 + lane; row < min(r0 + 32 * kLook, p.num_tokens); row += 32) {
+          if ((uint64_t)(__ldg(p.slots + row) - slot0) >= (uint64_t)bs || (uint32_t)(row - t) < (uint32_t)n) continue;
+          hit = true;
+          earlier |= row < t;
+        }
+        __syncwarp();
+      }
+      r0 += warp_rows;
+      if (r0 < p.num_tokens) look_at(p, r0, word);
+    }
+    apart = __syncthreads_or(hit);
+    if (apart && __syncthreads_or(earlier)) return;  // the block's first run stores this one's rows
+  }
+  if (!side.on) return;
+
+  float largest = 0.f;  // finite magnitude of the run
+  fold<T>(largest, v);
+#pragma unroll 1
+  for (int i = 32 + lane; i < run.count; i += 32) {
+    int c;
+    const int j = run.row(i, &c);
+    fold<T>(largest, run.load(j, c));
+  }
+  const bool odd = __any_sync(kAll, !(largest <= kFloatMax));
+  largest = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(largest)));
+  const float old = anew || !(stored > 0.f) ? 0.f : stored;
+  const float now = next_scale(old, largest);
+  const float inv = now > 0.f ? __frcp_rn(now) : 0.f;
+  if (apart || odd || !(__fmul_rn(largest, inv) < 127.5f)) {
+    store_slowly<T>(p, side.is_v, side.h, blk, t, apart);
+    return;
+  }
+  const int D = p.head_dim;
+  int8_t* block = side.cache + ((int64_t)blk * p.num_heads + side.h) * (bs * D);
+  if (now > old && !anew) rescale_block(block, bs * D, __fmul_rn(old, inv), lane);  // the step grew
+  const uint32_t* low = reinterpret_cast<const uint32_t*>(p.slots + t);  // low words of the slots
+  auto place = [&](int j, int c) -> int8_t* {
+    return block + ((__ldg(low + 2 * j) - (uint32_t)blk * (uint32_t)bs) * D + c * kVec);
+  };
+  if (lane < run.count) put<T>(place(j0, c0), v, inv);
+#pragma unroll 1
+  for (int i = 32 + lane; i < run.count; i += 32) {
+    int c;
+    const int j = run.row(i, &c);
+    put<T>(place(j, c), run.load(j, c), inv);
+  }
+  if (lane == 0) *scale_at = now;
 }
 
 // a / b, with the inverse 2^32 / b rounded up: their product is one too many at most.
@@ -445,18 +708,20 @@ int vfl_reshape_and_cache_int8(const void* key, const void* value, void* k_cache
   const int most = block_size < kMaxWindow ? block_size : kMaxWindow;
   const int64_t fit = ceil_div(num_tokens * 2 * num_heads, (int64_t)kNumSMs * 256);
   p.window = static_cast<int>(fit < most ? fit : most);
-  const int64_t warps = ceil_div(num_tokens, (int64_t)p.window) * 2 * num_heads;
-  const int64_t ctas = ceil_div(warps, (int64_t)kWarps);
-  if (warps > INT32_MAX) return fail(VFL_ERR_UNSUPPORTED, "reshape_and_cache_int8: too many tokens");
+  // the CTAs of a window share its heads evenly
+  p.parts = ceil_div(2u * num_heads, (uint32_t)kWarps);
+  const unsigned threads = 32 * ceil_div(2u * num_heads, p.parts);
+  const int64_t ctas = ceil_div(num_tokens, (int64_t)p.window) * p.parts;
+  if (num_heads > INT32_MAX / 4 || ctas > INT32_MAX) return fail(VFL_ERR_UNSUPPORTED, "reshape_and_cache_int8: too many tokens");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool even = 32 % row_pieces == 0;
   auto pick = [&](auto type) {
     using T = decltype(type);
-    if (p.window == 1) return even ? append_int8_kernel<T, true, true> : append_int8_kernel<T, false, true>;
-    return even ? append_int8_kernel<T, true, false> : append_int8_kernel<T, false, false>;
+    if (p.window == 1) return append_int8_row_kernel<T>;
+    return even ? append_int8_kernel<T, true> : append_int8_kernel<T, false>;
   };
   auto kern = dtype == VFL_DTYPE_F32 ? pick(float()) : pick(__nv_bfloat16());
-  kern<<<(unsigned)ctas, kThreads, 0, s>>>(p);
+  kern<<<(unsigned)ctas, threads, 0, s>>>(p);
   return cuda_status(cudaGetLastError(), "reshape_and_cache_int8 launch");
 }
 

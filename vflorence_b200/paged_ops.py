@@ -677,9 +677,9 @@ def reshape_and_cache_int8(key: torch.Tensor, value: torch.Tensor, k_cache: torc
     head_dim] and one float32 scale for each block and head, value = code * scale.
 
     A block's scale is its largest magnitude / 127. It grows when a larger token arrives (the
-    codes it holds are then rounded to the new step), and starts anew with the block's first slot.
-    Each run of consecutive rows in one block is rounded once, so write a block's tokens as
-    neighbouring rows. Infinities and NaNs are held to +-127 steps and 0, and flagged
+    codes it holds are then rounded to the new step), and starts anew in a call that writes the
+    block's first slot. The order of the rows changes nothing, but a block's tokens are stored
+    several times faster as neighbouring rows. Infinities and NaNs are held to +-127 steps and 0, and flagged
     (``read_device_errors``, DEVERR_NONFINITE)."""
     dev, n, h, bs, d = _int8_cache_checks(k_cache, v_cache, k_scale, v_scale)
     _require_cuda("key", key, dev)
