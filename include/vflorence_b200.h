@@ -421,8 +421,9 @@ int vfl_plan_attention_int8_shape(vfl_attention_int8_plan* plan, int warps, int 
 
 /* As vfl_attention_with_kv_cache, over the 8-bit cache. Query head h reads K/V head
  * h / (num_heads / num_kv_heads). Sums, softmax statistics and the output before its last
- * rounding are float32. A V scale of 0 says that the block's codes are 0 (as the append leaves
- * them); V scales below 2^-100 count as 2^-100. */
+ * rounding are float32. V scales below 2^-100, and those 2^90 times smaller than another of the
+ * context, may count as up to that much; so do scales of 0, whose blocks' codes are 0 (as the append
+ * leaves them). */
 int vfl_attention_with_kv_cache_int8(const vfl_attention_int8_plan* plan, const void* query,
                                      int64_t query_token_stride, const void* k_cache,
                                      const void* v_cache, const float* k_scale,

@@ -1,0 +1,80 @@
+"""The 8-bit attention's error where scales, weights or query elements of one row differ by much:
+against the 64-bit definition, with the head's own values as the measure."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from vflorence_b200 import paged_ops as ops
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def exact(q, cache, lens, table, scale):
+    """One row a request: (output, largest visible |v| of each head) in 64 bits."""
+    kc, vc, ks, vs = (t.double() for t in cache)
+    group, bs = q.shape[1] // kc.shape[1], kc.shape[2]
+    out, top = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape[:2], dtype=torch.float64)
+    for r, n in enumerate(lens.tolist()):
+        blocks = table[r, : -(-n // bs)].long()
+        k, v = ((c[blocks] * s[blocks][..., None, None]).transpose(0, 1).flatten(1, 2)[:, :n] for c, s in ((kc, ks), (vc, vs)))
+        for h in range(q.shape[1]):
+            out[r, h] = torch.softmax((k[h // group] @ q[r, h].double()) * scale, 0) @ v[h // group]
+            top[r, h] = v[h // group].abs().max()
+    return out, top
+
+
+def attend(q, cache, lens, table, scale, warps=0, splits=0):
+    starts = torch.arange(len(lens) + 1, dtype=torch.int32)
+    meta = ops.get_scheduler_metadata_int8(len(lens), q.shape[1], cache[0].shape[1], q.shape[2], lens, q.dtype, starts,
+                                           False, cache[0].shape[2])
+    if warps or splits:
+        ops.set_shape_int8(meta, warps, splits)
+    out = torch.full_like(q, 7.0).cuda()
+    ops.attention_with_kv_cache_int8(q.cuda(), *[t.cuda() for t in cache], out, starts.cuda(), lens.cuda(), scale, False,
+                                     table.cuda(), meta)
+    return out.cpu()
+
+
+def pool(lens, heads, d, bs, seed, v_scale):
+    g = torch.Generator().manual_seed(seed)
+    counts = [-(-n // bs) for n in lens]
+    n = sum(counts)
+    perm = torch.randperm(n, generator=g).to(torch.int32)
+    table = torch.zeros((len(lens), max(counts)), dtype=torch.int32)
+    at = 0
+    for r, c in enumerate(counts):
+        table[r, :c] = perm[at:at + c]
+        at += c
+    kc, vc = (torch.randint(-127, 128, (n, heads, bs, d), generator=g, dtype=torch.int8) for _ in range(2))
+    ks = (0.5 + torch.rand((n, heads), generator=g)) * 0.02
+    vs = (0.5 + torch.rand((n, heads), generator=g)) * v_scale
+    return g, [kc, vc, ks, vs], torch.tensor(lens, dtype=torch.int32), table
+
+
+def assert_within(got, want, top, dtype):
+    """bfloat16: the output's rounding (2^-9 of itself) and the weights' (2^-11 each). float32: the
+    exponent of a score of about 10 is off by a few 2^-24 of it."""
+    tol = 2.0 ** -10 * top[..., None] + 2.0 ** -8 * want.abs() if dtype == BF16 else 1e-5 * top[..., None]
+    over = (got.double() - want).abs() / tol
+    assert bool((over <= 1).all()), over.max().item()
+
+
+@pytest.mark.parametrize("warps,splits", [(0, 0), (1, 1), (2, 1), (4, 1), (2, 4), (1, 24)])
+@pytest.mark.parametrize("v_scale", [1e-3, 1e-5, 1e-8, 2.0 ** -98])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_zero_v_blocks_among_small_scales(dtype, v_scale, warps, splits):
+    """Blocks of zeros (scale 0, as the append leaves them) weigh in the sum of the weights alone."""
+    g, cache, lens, table = pool([592, 100, 2000], 2, 64, 16, 3, v_scale)
+    q = torch.randn((3, 2, 64), generator=g).to(dtype)
+    for r, n in enumerate(lens.tolist()):
+        for col in (0, 3, (n - 1) // 16):
+            cache[3][table[r, col]] = 0.0
+            cache[1][table[r, col]] = 0
+    want, top = exact(q, cache, lens, table, 0.125)
+    assert_within(attend(q, cache, lens, table, 0.125, warps, splits), want, top, dtype)

@@ -49,7 +49,8 @@ namespace {
 constexpr int kMaxWarps = 4;
 constexpr int kMaxCluster = 8;
 constexpr int kSmemPerSM = 227 * 1024;
-constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: smaller V scales count as it
+constexpr float kMinScale = 7.888609052210118e-31f;     // 2^-100: smaller V scales count as it
+constexpr float kScaleRange = 8.077935669463161e-28f;   // 2^-90: also those this much below the largest
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;
 
@@ -224,10 +225,11 @@ __device__ __forceinline__ void add_scaled(float4& o, float f, const float4& v) 
   o.w = fmaf(f, v.w, o.w);
 }
 
-// Factor of a piece with maximum `m` in a sum with maximum `m_all`. A piece without a maximum
-// holds zeros (nothing visible) or NaNs (every score a NaN), and either is to be kept.
-__device__ __forceinline__ float merge_factor(float m, float m_all) {
-  return m == -INFINITY ? 1.f : exp2_approx(m - m_all);
+// Root of the factor of a piece with maximum `m` in a sum with maximum `m_all`. The sums of weights take
+// it twice: theirs may be within range where the factor is not (blocks of zeros before others). A piece
+// without a maximum holds zeros (nothing visible) or NaNs (every score a NaN), and either is to be kept.
+__device__ __forceinline__ float merge_root(float m, float m_all) {
+  return m == -INFINITY ? 1.f : exp2_approx(0.5f * (m - m_all));
 }
 
 // First dim of word `w` (4 dims) of a row that lane group thread tq holds: whole groups of 64 dims
@@ -460,9 +462,9 @@ struct Sums {
           for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
           float& mr = m[nt][e];
           if (mx > mr + kRescaleSlack) {
-            const float alpha = mr == -INFINITY ? 0.f : exp2_approx(mr - mx);
+            const float root = mr == -INFINITY ? 0.f : exp2_approx(0.5f * (mr - mx)), alpha = root * root;
             mr = mx;
-            l[nt][e] *= alpha;
+            l[nt][e] = l[nt][e] * root * root;
 #pragma unroll
             for (int t = 0; t < S::kTiles; ++t) {
               acc[nt][t][e] *= alpha;
@@ -601,8 +603,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<T, D, NT>::kMinCtas) pag
 
   // ---- the tiles' scales: (ks, log2 vs, 1 / vs), 64 tiles of them in shared memory
   float4* meta = reinterpret_cast<float4*>(smem + region) + warp * 64;
-  float ks_next = 0.f, vs_next = 1.f;
+  float ks_next = 0.f, vs_next = 0.f, largest_vs = 0.f;
   auto load_scales = [&](int i, int at) {
+    ks_next = vs_next = 0.f;
     if (i < count) {
       const int row = tpb == 1 ? at : at / tpb;
       ks_next = __ldg(p.k_scale + row);
@@ -610,7 +613,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<T, D, NT>::kMinCtas) pag
     }
   };
   auto keep_scales = [&](int i) {
-    const float vs = vs_next > 0.f ? fmaxf(vs_next, kMinScale) : 1.f;  // a zero scale's codes are zeros
+    // A block of zeros has scale 0. Its tokens weigh in the sum of the weights alone: with a scale far
+    // below the others' they leave the maximum to the blocks that the output comes from, and their weights
+    // are still within range of it.
+    largest_vs = fmaxf(largest_vs, __uint_as_float(__reduce_max_sync(
+        0xffffffffu, vs_next > 0.f && vs_next <= FLT_MAX ? __float_as_uint(vs_next) : 0u)));
+    const float vs = fmaxf(vs_next, fmaxf(kMinScale, largest_vs * kScaleRange));
     meta[i & 63] = make_float4(ks_next, log2f(vs), 1.f / vs, 0.f);
   };
   load_scales(lane, place);
@@ -702,8 +710,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<T, D, NT>::kMinCtas) pag
 #pragma unroll
     for (int w = 0; w < kMaxWarps; ++w)
       if (w < warps) {
-        f[w] = merge_factor(ml[(w * S::kRows + row) * 2], m);
-        l = fmaf(f[w], ml[(w * S::kRows + row) * 2 + 1], l);
+        const float root = merge_root(ml[(w * S::kRows + row) * 2], m);
+        f[w] = root * root;
+        l = fmaf(root, root * ml[(w * S::kRows + row) * 2 + 1], l);
       }
     auto sum_at = [&](int d) {
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -733,12 +742,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<T, D, NT>::kMinCtas) pag
 #pragma unroll
     for (int o = kMaxCluster / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     m = __shfl_sync(0xffffffffu, m, 0);
-    const float factor = lane < p.cluster ? merge_factor(part.x, m) : 0.f;
-    float l = lane < p.cluster ? factor * part.y : 0.f;
+    const float root = lane < p.cluster ? merge_root(part.x, m) : 0.f;
+    float l = root * part.y * root;
 #pragma unroll
     for (int o = kMaxCluster / 2; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     l = __shfl_sync(0xffffffffu, l, 0);
-    if (lane < kMaxCluster) row_factor[warp * kMaxCluster + lane] = factor;
+    if (lane < kMaxCluster) row_factor[warp * kMaxCluster + lane] = root * root;
     __syncwarp();
     finish(row, m, l, [&](int d) {
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -772,9 +781,9 @@ __global__ void combine_int8_kernel(const Int8AttnParams p, int D) {
 #pragma unroll 4
     for (int s = 0; s < clusters; ++s) {
       const float2 ml = p.ws_ml[item + s];
-      const float f = merge_factor(ml.x, m);
-      l = fmaf(f, ml.y, l);
-      o = fmaf(f, p.ws_acc[(item + s) * D + d], o);
+      const float root = merge_root(ml.x, m);
+      l = fmaf(root, root * ml.y, l);
+      o = fmaf(root * root, p.ws_acc[(item + s) * D + d], o);
     }
     store_elem(static_cast<T*>(p.out) + row * p.out_stride + (int64_t)h * D + d, l == 0.f ? 0.f : o / l);
   }
