@@ -78,3 +78,48 @@ def test_zero_v_blocks_among_small_scales(dtype, v_scale, warps, splits):
             cache[1][table[r, col]] = 0
     want, top = exact(q, cache, lens, table, 0.125)
     assert_within(attend(q, cache, lens, table, 0.125, warps, splits), want, top, dtype)
+
+
+@pytest.mark.parametrize("lead", [4.0, 12.0, 60.0])
+@pytest.mark.parametrize("v_scale", [0.02, 1e-3, 1e-8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_zero_v_block_with_most_of_the_weight(dtype, v_scale, lead):
+    """A block of zeros whose scores lead by `lead`: the output is what is left for the others. Its
+    error is a share of itself, and no longer of the largest value."""
+    g, cache, lens, table = pool([700], 1, 64, 16, 5, v_scale)
+    q = torch.randn((1, 1, 64), generator=g).to(dtype)
+    b = int(table[0, 20])
+    cache[0][b, 0] = (q[0, 0].float() / q.float().abs().max() * 100).round().to(torch.int8)
+    cache[1][b], cache[3][b] = 0, 0.0
+    others = torch.ones(700, dtype=torch.bool)
+    others[20 * 16:21 * 16] = False
+    kc, ks = cache[0].double(), cache[2].double()
+    k = (kc[table[0].long()] * ks[table[0].long()][..., None, None]).transpose(0, 1).flatten(1, 2)[0, :700]
+    s = k @ q[0, 0].double() * 0.125
+    cache[2][b] = (float(s[others].max()) + lead) / float(kc[b, 0, 0] @ q[0, 0].double() * 0.125)
+    want, top = exact(q, cache, lens, table, 0.125)
+    got = attend(q, cache, lens, table, 0.125, 1, 1).double()
+    # the others' weights against one another, then the division: relative to the largest output,
+    # and the lead's own rounding, a few 2^-24 of a score of up to 80, times their sum
+    tol = (2.0 ** -7 if dtype == BF16 else 1e-4) * want.abs().max()
+    assert bool(((got - want).abs() <= tol).all()), ((got - want).abs().max() / want.abs().max()).item()
+
+
+@pytest.mark.parametrize("warps,splits", [(0, 0), (1, 1), (4, 1)])
+@pytest.mark.parametrize("n", [1024, 4096, 20000])
+def test_many_small_weights_beside_one_token(n, warps, splits):
+    """One token leads by 17.6; what thousands of tokens of one sign add is theirs alone (its own
+    values are 0). A weight is held to 2^-32 of the largest or better: n of them to n 2^-32."""
+    g, cache, lens, table = pool([n], 1, 64, 16, 9, 0.02)
+    cache[0].zero_()
+    cache[1].fill_(127)
+    cache[3].fill_(0.02)
+    q = torch.ones((1, 1, 64))
+    b, t = int(table[0, n // 40]), 5
+    cache[0][b, 0, t] = 100
+    cache[1][b, 0, t] = 0
+    cache[2][b] = 17.6 / (100 * 64 * 0.125)
+    want, top = exact(q, cache, lens, table, 0.125)
+    got = attend(q, cache, lens, table, 0.125, warps, splits).double()
+    tol = n * 2.0 ** -32 * top[..., None] + 1e-5 * want
+    assert bool(((got - want).abs() <= tol).all()), ((got - want).abs() / top[..., None]).max().item()

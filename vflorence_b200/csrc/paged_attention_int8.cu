@@ -5,9 +5,11 @@
 //     s_t = scale * ks_b * (q . kc_t),   out = sum_t e^(s_t) vs_b vc_t / sum_t e^(s_t).
 // A scale is one number for a tile of tokens, so neither product multiplies a cached element by
 // it: ks_b goes onto the score, and vs_b into the exponent. With base-2 scores s' = s log2 e and
-//     w_t = 2^(s'_t + log2 vs_b - M),  M the running maximum of s'_t + log2 vs_b,
-// out = sum w_t vc_t / sum (w_t / vs_b). Both sums and M are float32; w is at most 2^8 and is
-// rounded to half precision for its product alone (float32 queries: to a pair of halves).
+//     w_t = 2^(s'_t + log2 vs_b - M),  M below the running maximum of s'_t + log2 vs_b,
+// out = sum w_t vc_t / sum (w_t / vs_b). Both sums and M are float32. w is rounded to half precision for
+// its product alone (float32 queries: to a pair of halves, 2^-22 of it). M is kept 7 to 15 below the
+// maximum, so that the largest weight is near the upper end of a half's range and every weight is held
+// to 2^-32 of it or better: n tokens that small beside a large one are off by n 2^-32 of the largest |v|.
 //
 // Scores: K's codes enter m16n8k32 integer instructions as they are. A query row is brought to
 // whole numbers of 2^-14 (bfloat16) or 2^-22 (float32) of a power of two above its largest
@@ -52,7 +54,9 @@ constexpr int kSmemPerSM = 227 * 1024;
 constexpr float kMinScale = 7.888609052210118e-31f;     // 2^-100: smaller V scales count as it
 constexpr float kScaleRange = 8.077935669463161e-28f;   // 2^-90: also those this much below the largest
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescaleSlack = 8.f;
+constexpr float kLift = 7.f;            // log2 of the largest weight when its token sets the maximum
+constexpr float kRescaleSlack = 15.f;   // and the most before another one does: 2^15 is a half
+constexpr float kSumUnit = 0.000244140625f;  // 2^-12, of the sums of w / vs: 2^15 times 2^100 times a context's tokens is past float32
 
 struct Int8AttnParams {
   const void* q;
@@ -359,7 +363,7 @@ struct Query {
 template <typename T, int D, int NT>
 struct Sums {
   using S = Shape<T, D, NT>;
-  float m[NT][2], l[NT][2];
+  float m[NT][2], l[NT][2];  // l in units of 2^12
   float acc[NT][S::kTiles][4];
 
   __device__ __forceinline__ void reset() {
@@ -462,8 +466,9 @@ struct Sums {
           for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
           float& mr = m[nt][e];
           if (mx > mr + kRescaleSlack) {
-            const float root = mr == -INFINITY ? 0.f : exp2_approx(0.5f * (mr - mx)), alpha = root * root;
-            mr = mx;
+            const float to = mx - kLift;
+            const float root = mr == -INFINITY ? 0.f : exp2_approx(0.5f * (mr - to)), alpha = root * root;
+            mr = to;
             l[nt][e] = l[nt][e] * root * root;
 #pragma unroll
             for (int t = 0; t < S::kTiles; ++t) {
@@ -479,7 +484,7 @@ struct Sums {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = exp2_approx(x[e]);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) l[nt][e] = fmaf(x[e] + x[e + 2], mt.z, l[nt][e]);
+      for (int e = 0; e < 2; ++e) l[nt][e] = fmaf((x[e] + x[e + 2]) * kSumUnit, mt.z, l[nt][e]);
 #pragma unroll
       for (int term = 0; term < S::kTerms; ++term) {
         pb[nt][term][0] = transpose8(pack_half2(x[0], x[1]));
@@ -692,9 +697,10 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<T, D, NT>::kMinCtas) pag
       T* dst = static_cast<T*>(p.out) + out_row * p.out_stride + (int64_t)head * D;
       // l is a NaN where a score was: the row then is one, as in a plain softmax
       const float inv = l == 0.f ? 0.f : 1.f / l;
+      constexpr float c = kSumUnit;
       for (int d = lane * 4; d < D; d += 128) {
         const float4 o = sum_at(d);
-        store4(dst + d, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        store4(dst + d, o.x * inv * c, o.y * inv * c, o.z * inv * c, o.w * inv * c);
       }
     } else {
       const int64_t item = (out_row * p.num_heads + head) * clusters + split / p.cluster;
@@ -785,7 +791,7 @@ __global__ void combine_int8_kernel(const Int8AttnParams p, int D) {
       l = fmaf(root, root * ml.y, l);
       o = fmaf(root * root, p.ws_acc[(item + s) * D + d], o);
     }
-    store_elem(static_cast<T*>(p.out) + row * p.out_stride + (int64_t)h * D + d, l == 0.f ? 0.f : o / l);
+    store_elem(static_cast<T*>(p.out) + row * p.out_stride + (int64_t)h * D + d, l == 0.f ? 0.f : o / l * kSumUnit);
   }
 }
 
