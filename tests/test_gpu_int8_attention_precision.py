@@ -123,3 +123,19 @@ def test_many_small_weights_beside_one_token(n, warps, splits):
     got = attend(q, cache, lens, table, 0.125, warps, splits).double()
     tol = n * 2.0 ** -32 * top[..., None] + 1e-5 * want
     assert bool(((got - want).abs() <= tol).all()), ((got - want).abs() / top[..., None]).max().item()
+
+
+@pytest.mark.parametrize("d", [32, 64, 80, 128, 256])
+@pytest.mark.parametrize("ratio", [64.0, 1000.0])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_one_large_channel_in_the_query(dtype, ratio, d):
+    """A query channel `ratio` times the others whose cached keys are small (0 or one step): the
+    others' products decide the scores."""
+    g, cache, lens, table = pool([300, 40, 150], 2, d, 16, 11, 0.02)
+    q = torch.randn((3, 4, d), generator=g)
+    q[..., 1] = ratio
+    q = q.to(dtype)
+    cache[0][..., 1] = torch.randint(-1, 2, cache[0].shape[:-1], generator=g).to(torch.int8)
+    scale = 4.0 / (0.02 * 73.0 * math.sqrt(d))  # scores of the others of about 4
+    want, top = exact(q, cache, lens, table, scale)
+    assert_within(attend(q, cache, lens, table, scale), want, top, dtype)

@@ -12,10 +12,11 @@
 // to 2^-32 of it or better: n tokens that small beside a large one are off by n 2^-32 of the largest |v|.
 //
 // Scores: K's codes enter m16n8k32 integer instructions as they are. A query row is brought to
-// whole numbers of 2^-14 (bfloat16) or 2^-22 (float32) of a power of two above its largest
-// element, held as 2 or 3 planes of 8 bits: bfloat16 elements down to 2^-7 of the row's largest
-// are exact, what is smaller is rounded to 2^-15 of it, next to the output's 2^-9. The sums are
-// exact integers. Outputs: V's codes are exact in half precision and meet w in m16n8k16 half
+// whole numbers of 2^-22 (bfloat16) or 2^-30 (float32) of a power of two above its largest
+// element, held as 3 or 4 planes of 8 bits: elements down to 2^-15 (2^-7) of the row's largest are
+// exact, smaller ones are rounded to 2^-23 (2^-31) of that power, 13 (21) bits beside a channel a
+// thousand times larger. The sums are exact integers. A plane less takes 1 to 8 % off the times below
+// and leaves 5 (13) bits. Outputs: V's codes are exact in half precision and meet w in m16n8k16 half
 // instructions with float32 sums.
 //
 // Bound: HBM, 2 D bytes a token and K/V head, and close behind it the integer pipe that turns V's
@@ -150,6 +151,14 @@ __device__ __forceinline__ void mma_int_k32(int (&c)[4], uint32_t a0, uint32_t a
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The first of a chain: its sums start at `from`.
+__device__ __forceinline__ void mma_int_k32_from(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                 uint32_t b0, uint32_t b1, int from) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(from));
+}
 __device__ __forceinline__ void mma_int_k16(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
                : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
@@ -179,7 +188,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 template <typename T, int D, int NT>
 struct Shape {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kPlanes = sizeof(T) == 4 ? 3 : 2;  // 8-bit digits of a query element
+  static constexpr int kPlanes = sizeof(T) == 4 ? 4 : 3;  // 8-bit digits of a query element
   static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;   // halves that make up a weight
   static constexpr int kWords = D / 16;                   // 4-dim words a lane holds of a row
   static constexpr int kTiles = D / 16;                   // m16 tiles of the output
@@ -314,7 +323,7 @@ struct Query {
       const bool bad = ((__ballot_sync(0xffffffffu, odd) >> (ln.lane & ~3)) & 15u) != 0;  // in this lane's row
       // 2^e > amax >= 2^(e-1), from the exponent bits
       const int e = max(-90, static_cast<int>(__float_as_uint(amax) >> 23) - 126);
-      constexpr int kBits = S::kPlanes == 3 ? 22 : 14;
+      constexpr int kBits = 8 * S::kPlanes - 2;
       const float to_int = power_of_two(kBits - e);
 #pragma unroll
       for (int w = 0; w < S::kWords; ++w) {
@@ -324,17 +333,20 @@ struct Query {
           v[0] = v[1] = v[2] = v[3] = 0.f;
           if (on) load4(src + k_dim<D>(w, ln.tq), v);
         }
-        // adding 1.5 * 2^23 leaves the whole number in the sum's mantissa. Its digits base 256 in
-        // [-128, 127]: with 128 added to each they are the bytes of a plain number, and a byte
-        // loses the 128 again by flipping its top bit
-        constexpr uint32_t kBias = S::kPlanes == 3 ? 0x808080u : 0x8080u;
+        // digits base 256 in [-128, 127]: with 128 added to each they are the bytes of a plain number, and
+        // a byte loses the 128 again by flipping its top bit. Up to 2^22 adding 1.5 * 2^23 leaves the
+        // whole number in the sum's mantissa
+        constexpr uint32_t kBias = S::kPlanes == 4 ? 0x80808080u : 0x808080u;
         uint32_t c[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          c[i] = (__float_as_uint(fmaf(v[i], to_int, 12582912.f)) - 0x4b400000u + kBias) ^ kBias;
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t whole = S::kPlanes == 4 ? (uint32_t)__float2int_rn(v[i] * to_int)
+                                                 : __float_as_uint(fmaf(v[i], to_int, 12582912.f)) - 0x4b400000u;
+          c[i] = (whole + kBias) ^ kBias;
+        }
 #pragma unroll
         for (int plane = 0; plane < S::kPlanes; ++plane) {
-          constexpr uint32_t kPick[3] = {0x0040, 0x0051, 0x0062};  // byte 0, 1, 2 of two words
+          constexpr uint32_t kPick[4] = {0x0040, 0x0051, 0x0062, 0x0073};  // byte 0, 1, 2, 3 of two words
           const uint32_t pick = kPick[S::kPlanes - 1 - plane];
           const uint32_t packed = __byte_perm(__byte_perm(c[0], c[1], pick), __byte_perm(c[2], c[3], pick), 0x5410);
           const int at = (nt * S::kPlanes + plane) * S::kWords + w;
@@ -394,20 +406,25 @@ struct Sums {
                                        const Query<T, D, NT>& q, const Lane& ln) {
     const int tq = ln.tq, krow = ln.krow;
     // ---- scores: c[0..1] token krow of rows 2 tq, 2 tq + 1; c[2..3] token krow + 1
+    // A plane's sum is below 2^22 up to 256 dims: started at the bits of 1.5 * 2^23, it is that float's mantissa,
+    // and a subtraction turns it into a number where a conversion runs at a quarter of the rate (512 x 577
+    // float32 125 -> 121 us; bfloat16, with fewer planes, 103 -> 106). Otherwise the two highest planes are
+    // converted as one integer (2^14 * 127 * 512 < 2^31).
+    constexpr bool kMantissa = sizeof(T) == 4 && D <= 256;
+    constexpr int kFrom = kMantissa ? 0x4b400000 : 0;
+    auto number = [](int sum) { return kMantissa ? __int_as_float(sum) - 12582912.f : (float)sum; };
     int si[NT][S::kPlanes][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int pl = 0; pl < S::kPlanes; ++pl)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) si[nt][pl][e] = 0;
     constexpr int k64 = D / 64, k32 = (D % 64) / 32, k16 = (D % 32) / 16;
     auto pair = [&](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, int w) {  // words w, w + 1
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int pl = 0; pl < S::kPlanes; ++pl)
-          mma_int_k32(si[nt][pl], a0, a1, a2, a3, q.word(nt, pl, w, ln.lane), q.word(nt, pl, w + 1, ln.lane));
+        for (int pl = 0; pl < S::kPlanes; ++pl) {
+          if (w == 0)
+            mma_int_k32_from(si[nt][pl], a0, a1, a2, a3, q.word(nt, pl, w, ln.lane), q.word(nt, pl, w + 1, ln.lane), kFrom);
+          else
+            mma_int_k32(si[nt][pl], a0, a1, a2, a3, q.word(nt, pl, w, ln.lane), q.word(nt, pl, w + 1, ln.lane));
+        }
     };
 #pragma unroll
     for (int c = 0; c < k64; ++c) {
@@ -430,14 +447,16 @@ struct Sums {
         for (int pl = 0; pl < S::kPlanes; ++pl)
           mma_int_k16(si[nt][pl], a, b, q.word(nt, pl, 4 * k64 + 2 * k32, ln.lane));
     }
-    // digits to scores: the two highest planes fit an integer (2^14 * 127 * 512 < 2^31)
+    // digits to scores
     float sc[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        sc[nt][e] = (float)(si[nt][0][e] * 256 + si[nt][1][e]);
-        if (S::kPlanes == 3) sc[nt][e] = fmaf(sc[nt][e], 256.f, (float)si[nt][S::kPlanes - 1][e]);
+        sc[nt][e] = kMantissa ? fmaf(number(si[nt][0][e]), 256.f, number(si[nt][1][e]))
+                              : (float)(si[nt][0][e] * 256 + si[nt][1][e]);
+#pragma unroll
+        for (int pl = 2; pl < S::kPlanes; ++pl) sc[nt][e] = fmaf(sc[nt][e], 256.f, number(si[nt][pl][e]));
       }
 
     // ---- weights
@@ -798,7 +817,7 @@ __global__ void combine_int8_kernel(const Int8AttnParams p, int D) {
 // Dynamic shared memory of a CTA, as the kernel lays it out.
 int smem_bytes(int dtype, int D, int rows, int warps) {
   const int ring = warps * 32 * D * (D <= 128 ? 4 : 2), merge = (warps + 1) * rows * (D + 2) * 4;
-  const int words = (dtype == VFL_DTYPE_F32 ? 3 : 2) * rows / 8 * (D / 16);
+  const int words = (dtype == VFL_DTYPE_F32 ? 4 : 3) * rows / 8 * (D / 16);
   return (ring > merge ? ring : merge) + warps * 64 * 16 + (words > 32 ? words * 128 : 0);
 }
 
