@@ -105,6 +105,17 @@ def test_a_zero_v_block_with_most_of_the_weight(dtype, v_scale, lead):
     assert bool(((got - want).abs() <= tol).all()), ((got - want).abs().max() / want.abs().max()).item()
 
 
+def test_a_nan_scale_shows():
+    """A V or K block whose scale is a NaN makes the rows that see it NaN, and no others."""
+    for which in (2, 3):
+        g, cache, lens, table = pool([100, 90], 2, 64, 16, 7, 0.02)
+        q = torch.randn((2, 2, 64), generator=g).to(BF16)
+        cache[which][table[0, 2], 1] = math.nan
+        got = attend(q, cache, lens, table, 0.125)
+        assert got[0, 1].isnan().all()
+        assert got[0, 0].isfinite().all() and got[1].isfinite().all()
+
+
 @pytest.mark.parametrize("warps,splits", [(0, 0), (1, 1), (4, 1)])
 @pytest.mark.parametrize("n", [1024, 4096, 20000])
 def test_many_small_weights_beside_one_token(n, warps, splits):

@@ -642,7 +642,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<T, D, NT>::kMinCtas) pag
     // are still within range of it.
     largest_vs = fmaxf(largest_vs, __uint_as_float(__reduce_max_sync(
         0xffffffffu, vs_next > 0.f && vs_next <= FLT_MAX ? __float_as_uint(vs_next) : 0u)));
-    const float vs = fmaxf(vs_next, fmaxf(kMinScale, largest_vs * kScaleRange));
+    const float least = fmaxf(kMinScale, largest_vs * kScaleRange);
+    const float vs = vs_next < least ? least : vs_next;  // a NaN stays one
     meta[i & 63] = make_float4(ks_next, log2f(vs), 1.f / vs, 0.f);
   };
   load_scales(lane, place);
