@@ -1054,7 +1054,7 @@ int vfl_attention_with_kv_cache_int8(const vfl_attention_int8_plan* plan, const 
                                      void* stream) {
   int st = check_plan(plan);
   if (st) return st;
-  if (plan->num_reqs == 0 || plan->total_q == 0) return VFL_OK;
+  if (plan->num_reqs == 0 || plan->max_q_len == 0) return VFL_OK;  // rows before the first request's are nobody's
   if (!query || !k_cache || !v_cache || !k_scale || !v_scale || !output || !query_start_loc || !seq_lens ||
       (!block_table && table_cols > 0))
     return fail(VFL_ERR_INVALID_ARGUMENT, "attention_int8: NULL pointer");
