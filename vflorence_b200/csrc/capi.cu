@@ -88,6 +88,9 @@ int ensure_smem_attribute(const void* func, int bytes, int* done_flags) {
   if (st) return st;
   if (dev < 0 || dev >= kMaxDevices) return fail(VFL_ERR_CUDA, "device ordinal %d out of range", dev);
   if (__atomic_load_n(&done_flags[dev], __ATOMIC_ACQUIRE) >= bytes) return VFL_OK;
+  // threads that launch one kernel with several sizes: the limit only grows
+  std::lock_guard<std::mutex> lock(g_setup_mutex);
+  if (__atomic_load_n(&done_flags[dev], __ATOMIC_RELAXED) >= bytes) return VFL_OK;
   st = cuda_status(cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
                    "cudaFuncSetAttribute(max dynamic shared memory)");
   if (st) return st;
