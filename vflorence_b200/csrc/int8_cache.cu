@@ -318,9 +318,9 @@ __device__ __forceinline__ void put(int8_t* to, const uint4& w, float inv) {
 //
 // kEven: a row's pieces divide the warp, so a lane's pieces are a fixed step of rows apart.
 //
-// Measured: 64 x 585 tokens of 12 x 64 bfloat16 64 us, 172 MB at 2.7 TB/s: the instructions of a run (some
-// 600 for 16 rows) at about half a clock and scheduler are the bound, and the registers (64, for four CTAs
-// an SM; three with 80: 59, but 2000 single tokens of 16 x 64 48 instead of 45) what keeps them from more.
+// Measured: 64 x 585 tokens of 12 x 64 bfloat16 64 us, 172 MB at 2.7 TB/s: the instructions (780 a run of
+// 16 rows, 0.68 a clock and scheduler) are the bound. 64 registers, for four CTAs an SM; three with 80:
+// 59 us, but 2000 single tokens of 16 x 64 48 instead of 45.
 // 64 x 576 without a partly filled block 59. The same 64 x 585 rows token by token of all requests, which
 // take the slow way block by block: 1.0 ms.
 template <typename T, bool kEven>
@@ -620,7 +620,7 @@ __device__ __forceinline__ void spread(const uint2& w, float scale, uint4* out) 
 
 // One thread per 8 codes of K and of V; rows without a slot read as zeros. Bound: HBM, by the
 // rows written (64 x 585 tokens of 12 x 64 bfloat16: 35.5 us for 172 MB, 4.9 TB/s; two or four places
-// a thread with their loads in flight together: 34 and 38).
+// a thread with their loads in flight together: 34 and 38, and slower for small calls and float32).
 template <typename T>
 __global__ void __launch_bounds__(kThreads) gather_int8_kernel(const GatherParams p) {
   const uint32_t i = blockIdx.x * kThreads + threadIdx.x;

@@ -15,7 +15,7 @@
 // whole numbers of 2^-22 (bfloat16) or 2^-30 (float32) of a power of two above its largest
 // element, held as 3 or 4 planes of 8 bits: elements down to 2^-15 (2^-7) of the row's largest are
 // exact, smaller ones are rounded to 2^-23 (2^-31) of that power, 13 (21) bits beside a channel a
-// thousand times larger. The sums are exact integers. A plane less takes 1 to 8 % off the times below
+// thousand times larger. The sums are exact integers. A plane less takes 3 to 8 % off the times below
 // and leaves 5 (13) bits. Outputs: V's codes are exact in half precision and meet w in m16n8k16 half
 // instructions with float32 sums.
 //
@@ -32,11 +32,11 @@
 // own tiles through its own ring of cp.async stages; the warps' partial sums meet in shared
 // memory at the end. Long contexts of few requests are cut over a cluster of up to 8 CTAs, whose
 // sums meet in distributed shared memory, and over more clusters where that is not enough: then
-// a dependent launch adds the clusters' pieces.
+// a second launch adds the clusters' pieces.
 //
-// Measured, bfloat16, head_dim 64: 256 requests of 1 to 4096 tokens x 16 heads 171 us, 1079 MB at 6.3
-// TB/s (0.98 of a plain copy); 64 requests of 585 x 12 heads, three rows each, 16 us (58 MB), one
-// request of 577 6 us: start, joins and drain.
+// Measured, bfloat16, head_dim 64: 256 requests of 1 to 4096 tokens x 16 heads 180 us, 1079 MB at 6.0
+// TB/s (0.93 of a plain copy; 0.68 of the issue slots); 64 requests of 585 x 12 heads, three rows each,
+// 17.5 us (58 MB), one request of 577 6.2 us: start, joins and drain.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -792,7 +792,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, Shape<T, D, NT>::kMinCtas) pag
 // one thread a dim.
 template <typename T>
 __global__ void combine_int8_kernel(const Int8AttnParams p, int D) {
-  griddep_wait();
   const RequestSpan req = request_span(p, blockIdx.x);
   if ((int)blockIdx.y >= req.rows) return;
   const int h = blockIdx.z;
@@ -846,12 +845,12 @@ void set_splits(vfl_attention_int8_plan* plan, int64_t splits) {
 // Warps and CTAs of an item. Measured on B200 (device time, bfloat16, head_dim 64; items = requests
 // x K/V heads x row chunks):
 //   * more items than slots: the CTA's start (about 5 us, five CTAs of four warps an SM) is spread
-//     over fewer warps. 8192 items of 9 tiles: 1, 2, 4 warps take 44, 53, 64 us; 4096 items of 32
-//     tiles: 63, 56, 60; 4096 of 128: 223, 187, 171. Hence one warp up to 16 tiles, two up to 64.
+//     over fewer warps. 8192 items of 9 tiles: 1, 2, 4 warps take 36, 49, 69 us; 4096 items of 32
+//     tiles: 54, 51, 60; 4096 of 1 to 256: 245, 198, 180. Hence one warp up to 16 tiles, two up to 64.
 //   * items that four warps run in little more than one wave, and two warps in one, run two (768
-//     items of 37 tiles: 16.6 against 20.5 us);
+//     items of 37 tiles: 17.4 against 20.8 us);
 //   * fewer items: the context is cut until the slots are full, over a cluster at most (one of 8
-//     takes 8.9 us for 16 items of 256 tiles, four clusters and the adding launch 10.1), past 512
+//     takes 9.1 us for 16 items of 256 tiles, four clusters and the adding launch 9.9), past 512
 //     tiles over more.
 void choose_shape(vfl_attention_int8_plan* plan, int64_t items, int64_t tiles_sum) {
   const int64_t mean = items > 0 ? tiles_sum / items : 0;
@@ -874,7 +873,7 @@ void choose_shape(vfl_attention_int8_plan* plan, int64_t items, int64_t tiles_su
     splits = splits < by_len ? splits : by_len;
     if (longest <= 512 && splits > kMaxCluster) splits = kMaxCluster;
     // clusters do not fill every GPC (with two CTAs an SM 71 of 4 and 33 of 8 were measured to fit):
-    // one more is a second wave (72 float32 items of 16 rows: 20 us over clusters of 4, 17 of 2)
+    // one more is a second wave (72 float32 items of 16 rows: 20.4 us over clusters of 4, 17 of 2)
     if (splits >= 8 && splits < 16 && 100 * items > 89 * (slots / 8)) splits = 4;
     if (splits >= 4 && splits < 8 && 100 * items > 96 * (slots / 4)) splits = 2;
   }

@@ -826,8 +826,8 @@ def linear_int4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias
                 activation: str | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """``act(x @ W.T + bias)`` with the 4-bit weight ``quantize_int4`` makes: x [rows, k] float32 or
     bfloat16 (unit column stride), codes uint8 [n, k // 2], scales [n, k // group_size] and bias [n] of x's
-    dtype; float32 sums, the exact GELU fused. For the few rows of a decode step (any number is
-    taken). Returns ``out`` (a new [rows, n] tensor when None)."""
+    dtype; float32 sums, the exact GELU fused. For the few rows of a decode step (any number is taken;
+    past 16 to 32 rows a bfloat16 GEMM over full weights is faster). Returns ``out`` (a new [rows, n] tensor when None)."""
     dev = codes.device
     _require_cuda("codes", codes, dev)
     _require_cuda("x", x, dev)
