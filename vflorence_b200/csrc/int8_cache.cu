@@ -18,7 +18,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kCtas = 4;        // of many rows, that an SM is to hold
 constexpr int kMaxWindow = 16;  // rows whose runs one warp stores, at most 31
 
 // Smallest scale kept: the attention divides by V scales, and 2^100 times a context's token
@@ -313,20 +312,29 @@ __device__ __forceinline__ void put(int8_t* to, const uint4& w, float inv) {
 // another row) has its CTA look through the slots of the call. So a block is written by one warp a head
 // and needs no lock, and the order of the rows changes nothing.
 
+// Pieces of a run that a lane holds in the wide variant, a block of 16 x 64 elements.
+template <typename T>
+__host__ __device__ constexpr int held_wide() {
+  return sizeof(T) == 4 ? 8 : 4;
+}
+
 // The runs of many rows: a warp takes those that begin in its window of rows. A run of up to kHeld pieces
 // a lane stays in registers from its maximum to its codes; a longer one is read a second time.
 //
 // kEven: a row's pieces divide the warp, so a lane's pieces are a fixed step of rows apart.
 //
-// Measured: 64 x 585 tokens of 12 x 64 bfloat16 64 us, 172 MB at 2.7 TB/s: the instructions (780 a run of
-// 16 rows, 0.68 a clock and scheduler) are the bound. 64 registers, for four CTAs an SM; three with 80:
-// 59 us, but 2000 single tokens of 16 x 64 48 instead of 45.
-// 64 x 576 without a partly filled block 59. The same 64 x 585 rows token by token of all requests, which
-// take the slow way block by block: 1.0 ms.
-template <typename T, bool kEven>
-__global__ void __launch_bounds__(kThreads, kCtas) append_int8_kernel(const __grid_constant__ AppendParams p) {
+// kWide: three CTAs an SM with 80 registers instead of four with 64, for prompts whose blocks are held
+// whole: 64 x 585 tokens of 12 x 64 bfloat16 59 us instead of 65, 64 x 576 float32 80 instead of 84; with
+// single rows (2000 of 16 x 64 bfloat16) 48 instead of 45, with blocks read twice (32 x 572 of 12 x 128 in
+// blocks of 32) 54 instead of 51.
+//
+// Measured: 64 x 585 tokens of 12 x 64 bfloat16 59 us, 172 MB at 2.9 TB/s: the instructions (640 a run of
+// 16 rows, 0.61 a clock and scheduler) are the bound. 64 x 576 without a partly filled block 55. The same
+// 64 x 585 rows token by token of all requests, which take the slow way block by block: 1.0 ms.
+template <typename T, bool kEven, bool kWide>
+__global__ void __launch_bounds__(kThreads, kWide ? 3 : 4) append_int8_kernel(const __grid_constant__ AppendParams p) {
   constexpr int kVec = Elem<T>::kVec;
-  constexpr int kHeld = 4;
+  constexpr int kHeld = kWide ? held_wide<T>() : 4;
   constexpr uint32_t kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
   const int t_begin = blockIdx.x / p.parts * p.window;
@@ -718,7 +726,10 @@ int vfl_reshape_and_cache_int8(const void* key, const void* value, void* k_cache
   auto pick = [&](auto type) {
     using T = decltype(type);
     if (p.window == 1) return append_int8_row_kernel<T>;
-    return even ? append_int8_kernel<T, true> : append_int8_kernel<T, false>;
+    // so many rows are prompts: their runs are whole blocks, here held in registers (see kWide)
+    if (p.window == kMaxWindow && (int64_t)block_size * row_pieces <= 32 * held_wide<T>())
+      return even ? append_int8_kernel<T, true, true> : append_int8_kernel<T, false, true>;
+    return even ? append_int8_kernel<T, true, false> : append_int8_kernel<T, false, false>;
   };
   auto kern = dtype == VFL_DTYPE_F32 ? pick(float()) : pick(__nv_bfloat16());
   kern<<<(unsigned)ctas, threads, 0, s>>>(p);
