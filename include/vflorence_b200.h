@@ -369,10 +369,10 @@ int vfl_fork_token_rows(int32_t* tokens, int64_t row_stride, int32_t num_rows, i
  *          starts anew) or when it is not above 0; a * (1/127) below 2^-100 counts as 0;
  *     codes the block holds become rint(code * (s * (1/s'))) when s' > s and it did not start anew;
  *     new codes are rint(x * (1/s')) held to [-127, 127], 0 when s' is 0.
- * Infinities are held to +-127 and NaNs to 0, flagged VFL_DEVERR_NONFINITE. The order of the tokens
- * changes nothing (but two tokens of one slot, of which either is kept); a block's tokens that are
- * not neighbours in the call take several times longer. Calls that write the same block are to be
- * ordered (one stream, or events).
+ * Infinities are held to +-127 and NaNs to 0, flagged VFL_DEVERR_NONFINITE. A call names a slot once.
+ * The order of the tokens changes nothing, but a block's tokens that are not neighbours in the call
+ * take several times longer. Calls that write the same block are to be ordered (one stream, or
+ * events).
  * head_dim a multiple of 16; pointers and token strides 16-byte aligned. */
 int vfl_reshape_and_cache_int8(const void* key, const void* value, void* k_cache, void* v_cache,
                                float* k_scale, float* v_scale, const int64_t* slot_mapping,

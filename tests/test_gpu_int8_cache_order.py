@@ -135,3 +135,34 @@ def test_the_same_codes_whatever_the_order_of_the_rows():
         results.append([x.cpu() for x in dev])
     for other in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+
+
+@pytest.mark.parametrize("share", [False, True])
+def test_many_runs_of_few_rows(share):
+    """Two rows a block, thousands of rows apart, replayed from a CUDA graph. `share`: the blocks' numbers
+    all meet in one table of those by which the runs are told apart, more than it holds."""
+    h, d, bs, blocks = 8, 16, 16, 4000
+    pool = torch.arange(1, 50000 if share else blocks + 1)
+    if share:
+        pool = pool[(pool * 2654435761 >> 12) % 8 == 5][:blocks]
+    assert pool.numel() == blocks
+    n = int(pool.max()) + 1
+    g = torch.Generator().manual_seed(1)
+    blk = torch.cat([pool[torch.randperm(blocks, generator=g)] for _ in range(2)])
+    off = torch.cat([torch.randint(1, 8, (blocks,), generator=g), torch.randint(8, 16, (blocks,), generator=g)])
+    key, value = (torch.randn((2 * blocks, h, d), generator=g).to(BF16).cuda() for _ in range(2))
+    blk, off = blk.cuda(), off.cuda()
+    codes = [torch.zeros((n, h, bs, d), dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros((n, h), device="cuda") for _ in range(2)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.reshape_and_cache_int8(key, value, *codes, *scales, blk * bs + off)
+    graph.replay()
+    for x, c, s in ((key, codes[0], scales[0]), (value, codes[1], scales[1])):
+        x = x.float()
+        a = torch.zeros((n, h), device="cuda").index_reduce_(0, blk, x.abs().amax(-1), "amax")
+        want_s = a * torch.tensor(1.0 / 127.0, device="cuda")
+        inv = torch.where(want_s > 0, 1.0 / want_s, 0.0)
+        want = torch.zeros_like(c)
+        want[blk, :, off] = (x * inv[blk][..., None]).round().clamp(-127, 127).to(torch.int8)
+        assert torch.equal(s, want_s) and torch.equal(c, want)

@@ -11,7 +11,11 @@
 //
 // Both kernels move bytes: the bound is HBM for many tokens and one dependent round trip (slot,
 // then the block's scale and the token) for a few.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace vfl {
 namespace {
@@ -36,6 +40,8 @@ struct AppendParams {
   uint32_t inverse;          // 2^32 / 16-byte pieces of a row, rounded up
   int rows_per_warp;         // 32 / pieces of a row
   uint32_t parts;            // CTAs that share a window's heads
+  int threads;               // of each
+  int block_mask;            // block_size - 1 where that is a power of two, else 0
   unsigned int* err;
 };
 
@@ -231,6 +237,16 @@ struct Side {
   }
 };
 
+// Where a run whose first slot is `slot` is told whose it is (see kRunAlone), for the CTAs of a part: in
+// the code row of that slot, of the head of the CTAs' first warp.
+__device__ __forceinline__ uint32_t* told_at(const AppendParams& p, int64_t slot, uint32_t part) {
+  const int first = part * (p.threads >> 5);
+  const int h = first < p.num_heads ? first : first - p.num_heads;
+  const int64_t blk = block_of(slot, p.block_size), off = slot - blk * p.block_size;
+  int8_t* cache = first < p.num_heads ? p.k_cache : p.v_cache;
+  return reinterpret_cast<uint32_t*>(cache + ((blk * p.num_heads + h) * p.block_size + off) * p.head_dim);
+}
+
 // Row t's block (-1: no slot, -2: a slot past the pool), whether it is the block's first slot, and the
 // slot less the row, which is the same all along a run in order.
 __device__ __forceinline__ int block_at(const AppendParams& p, int t, bool* opens, uint32_t* lead) {
@@ -308,14 +324,151 @@ __device__ __forceinline__ void put(int8_t* to, const uint4& w, float inv) {
 // filled by one call is rounded once.
 //
 // A block may have other rows in the call (time-major prompts; a padding row in a block's middle). Its
-// first run stores them all: every run that is not a whole block in order (which leaves no slot to
-// another row) has its CTA look through the slots of the call. So a block is written by one warp a head
-// and needs no lock, and the order of the rows changes nothing.
+// first run stores them all, unless a run is the whole block in order, which leaves no slot to another
+// row. So a block is written by one warp a head and needs no lock, and the order of the rows changes
+// nothing. Which run is whose is found out by a kernel before (many rows) or by the CTA that stores the
+// row (few).
 
-// Pieces of a run that a lane holds in the wide variant, a block of 16 x 64 elements.
-template <typename T>
-__host__ __device__ constexpr int held_wide() {
-  return sizeof(T) == 4 ? 8 : 4;
+// What a run that is not a whole block in order is told, in the first 4 bytes of code rows of its first
+// slot (see told_at). A CTA has read its word before it stores, and the bytes are written anew with the
+// run's codes. No code is -128: a run whose word the codes of another have overwritten is a later one.
+constexpr uint32_t kRunAlone = 0x80808001u;  // the block's only run
+constexpr uint32_t kRunFirst = 0x80808002u;  // the block has more
+constexpr uint32_t kRunLater = 0x80808000u;  // another run stores its rows
+
+constexpr int kRunsCluster = 8;
+constexpr int kRunsThreads = 1024;
+constexpr int kRunsPerCta = 2048;  // rows, and so runs at most, for which a launch has a CTA
+constexpr int kTableSize = 4096;   // blocks of a CTA's table
+constexpr int kListSize = 3584;    // its entries, and the runs of a CTA's list, at most
+
+// Tells the runs. A cluster looks at all slots, each CTA at a stretch of them, and keeps the runs of a
+// share of the blocks, by a hash of their numbers: each in the list of the CTA that met it, their blocks
+// with their first rows in the CTAs' tables. The launch after it reads its slots and rows meanwhile.
+//
+// Measured: 13 to 16 us alone (37000 to 60000 rows; 50 for 512 x 585), nearly all of it beside the launch
+// after it: an append of 3000 prompts of 20 tokens (12 x 64 bfloat16) takes 143 us, of 512 x 585 rows 466.
+// With each storing CTA looking through the slots, as for few rows, they took 318 and 520, and 64 x 585
+// rows 59 as they do here.
+__global__ void __cluster_dims__(kRunsCluster, 1, 1) __launch_bounds__(kRunsThreads)
+append_int8_runs_kernel(const __grid_constant__ AppendParams p) {
+  griddep_launch_dependents();
+  __shared__ int s_block[kTableSize], s_first[kTableSize];  // -1: no block
+  __shared__ uint32_t s_more[kTableSize / 32], s_whole[kTableSize / 32];  // has several runs; one in order
+  __shared__ int s_list[kListSize], s_count, s_used;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = cluster.block_rank(), lane = threadIdx.x & 31;
+  const uint32_t share = blockIdx.x / kRunsCluster, shares = gridDim.x / kRunsCluster;
+  const int bs = p.block_size;
+  for (int i = threadIdx.x; i < kTableSize; i += kRunsThreads) {
+    s_block[i] = -1;
+    s_first[i] = INT32_MAX;
+  }
+  for (int i = threadIdx.x; i < kTableSize / 32; i += kRunsThreads) s_more[i] = s_whole[i] = 0;
+  if (threadIdx.x == 0) s_count = s_used = 0;
+  cluster.sync();
+
+  auto slot_at = [&](int row) { return row >= 0 && row < p.num_tokens ? __ldg(p.slots + row) : -1; };
+  auto inside = [&](int64_t slot, int64_t slot0) { return (uint64_t)(slot - slot0) < (uint64_t)bs; };
+  auto hash_of = [](int blk) { return (uint32_t)blk * 2654435761u; };
+  auto table_of = [&](int blk) { return static_cast<int>(hash_of(blk) >> 12) & (kRunsCluster - 1); };  // whose it is in
+  // the entry of a block in a table: its own, or the free one where it is to be
+  auto entry_of = [&](const int* blocks, int blk) {
+    uint32_t i = (hash_of(blk) ^ (uint32_t)blk >> 9) % kTableSize;
+    for (;; i = (i + 1) % kTableSize) {
+      const int there = *const_cast<volatile const int*>(blocks + i);
+      if (there == -1 || there == blk) return i;
+    }
+  };
+
+  // this CTA's stretch
+  const int per = ceil_div(ceil_div(p.num_tokens, kRunsCluster), 32) * 32, r_begin = rank * per;
+  const int r_end = min(r_begin + per, p.num_tokens);
+  constexpr int kFlight = 4;
+  for (int r0 = r_begin + threadIdx.x; r0 - lane < r_end; r0 += kFlight * kRunsThreads) {
+    int64_t slot[kFlight], edge[kFlight];
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      const int row = r0 + u * kRunsThreads;
+      slot[u] = row < r_end ? slot_at(row) : -1;
+      edge[u] = lane == 0 ? slot_at(row - 1) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      int64_t before = __shfl_up_sync(0xffffffffu, slot[u], 1);
+      if (lane == 0) before = edge[u];
+      // a run goes on, most often, with the next slot of the block
+      if (slot[u] < 0 || slot[u] >= p.capacity || (slot[u] == before + 1 && p.block_mask && (slot[u] & p.block_mask))) continue;
+      const int blk = static_cast<int>(block_of(slot[u], bs));
+      if (inside(before, (int64_t)blk * bs) || __umulhi(hash_of(blk), shares) != share) continue;
+      const int at = atomicAdd(&s_count, 1);
+      if (at < kListSize) s_list[at] = r0 + u * kRunsThreads;
+    }
+  }
+  __syncthreads();
+
+  auto whole_block = [&](int row, int64_t slot, int64_t slot0) {  // the run that begins here is, in order, and ends
+    bool same = slot == slot0 && slot_at(row + bs - 1) == slot + bs - 1 && !inside(slot_at(row + bs), slot0);
+    for (int i = 1; i < bs - 1 && same; ++i) same = slot_at(row + i) == slot + i;
+    return same;
+  };
+  const int runs = min(s_count, kListSize);
+  for (int j = threadIdx.x; j < runs; j += kRunsThreads) {
+    const int row = s_list[j];
+    const int64_t slot = slot_at(row);
+    const int blk = static_cast<int>(block_of(slot, bs)), to = table_of(blk);
+    const bool whole = whole_block(row, slot, (int64_t)blk * bs);
+    if (whole) s_list[j] = -1;
+    // entries are counted before they are made, so that a table never fills up
+    if (atomicAdd(cluster.map_shared_rank(&s_used, to), 1) >= kListSize) continue;
+    int* blocks = cluster.map_shared_rank(s_block, to);
+    uint32_t i = entry_of(blocks, blk);
+    int old = atomicCAS(blocks + i, -1, blk);
+    while (old != -1 && old != blk) {  // another block took it
+      i = entry_of(blocks, blk);
+      old = atomicCAS(blocks + i, -1, blk);
+    }
+    atomicMin(cluster.map_shared_rank(s_first, to) + i, row);
+    if (old == blk) atomicOr(cluster.map_shared_rank(s_more, to) + i / 32, 1u << i % 32);
+    if (whole) atomicOr(cluster.map_shared_rank(s_whole, to) + i / 32, 1u << i % 32);
+  }
+  cluster.sync();
+
+  auto tell = [&](int64_t slot, uint32_t what) {
+    for (uint32_t part = 0; part < p.parts; ++part) __stcg(told_at(p, slot, part), what);
+  };
+  bool fits = true;
+  for (int c = 0; c < kRunsCluster; ++c)
+    fits &= *cluster.map_shared_rank(&s_count, c) <= kListSize && *cluster.map_shared_rank(&s_used, c) <= kListSize;
+  if (fits) {
+    for (int j = threadIdx.x; j < runs; j += kRunsThreads) {
+      const int row = s_list[j];
+      if (row < 0) continue;
+      const int64_t slot = slot_at(row);
+      const int blk = static_cast<int>(block_of(slot, bs)), in = table_of(blk);
+      const uint32_t i = entry_of(cluster.map_shared_rank(s_block, in), blk);
+      uint32_t what = kRunAlone;
+      if (cluster.map_shared_rank(s_more, in)[i / 32] >> i % 32 & 1)
+        what = cluster.map_shared_rank(s_first, in)[i] == row ? kRunFirst : kRunLater;
+      if (cluster.map_shared_rank(s_whole, in)[i / 32] >> i % 32 & 1) what = kRunLater;
+      tell(slot, what);
+    }
+  } else {  // more runs than that (their blocks' numbers meet in the hash): each looks for itself
+    for (int row = r_begin + threadIdx.x; row < r_end; row += kRunsThreads) {
+      const int64_t slot = slot_at(row);
+      if (slot < 0 || slot >= p.capacity) continue;
+      const int blk = static_cast<int>(block_of(slot, bs));
+      const int64_t slot0 = (int64_t)blk * bs;
+      if (__umulhi(hash_of(blk), shares) != share || inside(slot_at(row - 1), slot0) || whole_block(row, slot, slot0)) continue;
+      int end = row + 1;
+      while (inside(slot_at(end), slot0)) ++end;
+      uint32_t what = kRunAlone;
+      for (int j = 0; j < p.num_tokens && what != kRunLater; ++j)
+        if ((j < row || j >= end) && inside(slot_at(j), slot0)) what = j < row ? kRunLater : kRunFirst;
+      tell(slot, what);
+    }
+  }
+  cluster.sync();  // no CTA leaves while another still reads its table
 }
 
 // The runs of many rows: a warp takes those that begin in its window of rows. A run of up to kHeld pieces
@@ -323,18 +476,14 @@ __host__ __device__ constexpr int held_wide() {
 //
 // kEven: a row's pieces divide the warp, so a lane's pieces are a fixed step of rows apart.
 //
-// kWide: three CTAs an SM with 80 registers instead of four with 64, for prompts whose blocks are held
-// whole: 64 x 585 tokens of 12 x 64 bfloat16 59 us instead of 65, 64 x 576 float32 80 instead of 84; with
-// single rows (2000 of 16 x 64 bfloat16) 48 instead of 45, with blocks read twice (32 x 572 of 12 x 128 in
-// blocks of 32) 54 instead of 51.
-//
-// Measured: 64 x 585 tokens of 12 x 64 bfloat16 59 us, 172 MB at 2.9 TB/s: the instructions (640 a run of
-// 16 rows, 0.61 a clock and scheduler) are the bound. 64 x 576 without a partly filled block 55. The same
-// 64 x 585 rows token by token of all requests, which take the slow way block by block: 1.0 ms.
-template <typename T, bool kEven, bool kWide>
-__global__ void __launch_bounds__(kThreads, kWide ? 3 : 4) append_int8_kernel(const __grid_constant__ AppendParams p) {
+// Measured: 64 x 585 tokens of 12 x 64 bfloat16 60 us, 172 MB at 2.9 TB/s: the instructions (780 a run of
+// 16 rows, 0.73 a clock and scheduler) are the bound; 80 registers, for three CTAs an SM instead of four,
+// changed nothing. 2000 single rows of 16 x 64 46 us. The same 64 x 585 rows token by token of all
+// requests, which take the slow way block by block: 0.76 ms.
+template <typename T, bool kEven>
+__global__ void __launch_bounds__(kThreads, 4) append_int8_kernel(const __grid_constant__ AppendParams p) {
   constexpr int kVec = Elem<T>::kVec;
-  constexpr int kHeld = kWide ? held_wide<T>() : 4;
+  constexpr int kHeld = 4;
   constexpr uint32_t kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
   const int t_begin = blockIdx.x / p.parts * p.window;
@@ -371,58 +520,15 @@ __global__ void __launch_bounds__(kThreads, kWide ? 3 : 4) append_int8_kernel(co
     partial |= in_order && n == bs ? 0u : 1u << at;
   }
 
-  // other rows of these runs' blocks (bit i: of the run's at row t_begin - 1 + i), looked for by the CTA
+  // what these runs were told
   uint32_t apart = 0;
   if (partial != 0) {
-    constexpr int kLook = 16;
-    uint32_t hits = 0, earlier = 0;
-    // the warp's i-th chunk of rows: chunks go from the window's down to the first, then up
-    const int chunks = ceil_div(p.num_tokens, 32 * kLook), at_window = t_begin / (32 * kLook);
-    auto look = [&](int i) {
-      const int r0 = (i <= at_window ? at_window - i : i) * (32 * kLook);
-      uint32_t word[kLook];
-      look_at(p, r0, word);
-#pragma unroll 1
-      for (uint32_t left = partial; left != 0; left &= left - 1) {
-        const int at = __ffs(left) - 1;
-        const int t = t_begin - 1 + at, n = __shfl_sync(kAll, n_l, at);
-        const int64_t slot0 = (int64_t)__shfl_sync(kAll, blk_l, at) * bs;
-        if (__any_sync(kAll, may_hit(word, slot0, bs))) {  // the whole slots decide
-#pragma unroll 1
-          for (int row = r0 + lane; row < min(r0 + 32 * kLook, p.num_tokens); row += 32) {
-            if ((uint64_t)(__ldg(p.slots + row) - slot0) >= (uint64_t)bs || (uint32_t)(row - t) < (uint32_t)n) continue;
-            hits |= 1u << at;
-            earlier |= row < t ? 1u << at : 0u;
-          }
-          __syncwarp();
-        }
-      }
-    };
-    __shared__ uint32_t s_hits, s_earlier;
-    auto gather = [&]() {  // the CTA's bits, in every thread
-      if (!__syncthreads_or(hits != 0)) return;
-      if (threadIdx.x == 0) s_hits = s_earlier = 0;
-      __syncthreads();
-      atomicOr(&s_hits, hits);
-      atomicOr(&s_earlier, earlier);
-      __syncthreads();
-      hits = s_hits;
-      earlier = s_earlier;
-      __syncthreads();
-    };
-    const int warps = blockDim.x >> 5;
-    int i = threadIdx.x >> 5;
-    if (i < chunks) look(i);
-    if (chunks > warps) {  // rows of a block apart are near, most often: then this was enough for all but the first
-      gather();
-      if ((earlier & partial) != partial) {
-#pragma unroll 1
-        for (i += warps; i < chunks; i += warps) look(i);
-      }
-    }
-    gather();
-    starts &= ~earlier;  // a block's first run stores all its rows
-    apart = hits & ~earlier;
+    griddep_wait();
+    uint32_t told = 0;
+    if (partial >> lane & 1) told = __ldcg(told_at(p, __ldg(p.slots + t_begin - 1 + lane), blockIdx.x % p.parts));
+    apart = __ballot_sync(kAll, told == kRunFirst);
+    starts &= ~partial | apart | __ballot_sync(kAll, told == kRunAlone);
+    __syncthreads();  // every warp has read before one stores
   }
   if (!side.on) return;
 
@@ -493,6 +599,7 @@ __global__ void __launch_bounds__(kThreads, kWide ? 3 : 4) append_int8_kernel(co
     const int at = __ffs(slow) - 1;
     store_slowly<T>(p, side.is_v, side.h, __shfl_sync(kAll, blk_l, at), t_begin - 1 + at, apart >> at & 1);
   }
+  if (blockIdx.x == gridDim.x - 1) griddep_wait();  // this launch ends after the one before it
 }
 
 // Few rows, as in a decode step: a CTA has one row, whose run is most often itself, and eight CTAs share
@@ -716,9 +823,11 @@ int vfl_reshape_and_cache_int8(const void* key, const void* value, void* k_cache
   const int most = block_size < kMaxWindow ? block_size : kMaxWindow;
   const int64_t fit = ceil_div(num_tokens * 2 * num_heads, (int64_t)kNumSMs * 256);
   p.window = static_cast<int>(fit < most ? fit : most);
+  p.block_mask = (block_size & (block_size - 1)) == 0 ? block_size - 1 : 0;
   // the CTAs of a window share its heads evenly
   p.parts = ceil_div(2u * num_heads, (uint32_t)kWarps);
   const unsigned threads = 32 * ceil_div(2u * num_heads, p.parts);
+  p.threads = static_cast<int>(threads);
   const int64_t ctas = ceil_div(num_tokens, (int64_t)p.window) * p.parts;
   if (num_heads > INT32_MAX / 4 || ctas > INT32_MAX) return fail(VFL_ERR_UNSUPPORTED, "reshape_and_cache_int8: too many tokens");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -726,14 +835,27 @@ int vfl_reshape_and_cache_int8(const void* key, const void* value, void* k_cache
   auto pick = [&](auto type) {
     using T = decltype(type);
     if (p.window == 1) return append_int8_row_kernel<T>;
-    // so many rows are prompts: their runs are whole blocks, here held in registers (see kWide)
-    if (p.window == kMaxWindow && (int64_t)block_size * row_pieces <= 32 * held_wide<T>())
-      return even ? append_int8_kernel<T, true, true> : append_int8_kernel<T, false, true>;
-    return even ? append_int8_kernel<T, true, false> : append_int8_kernel<T, false, false>;
+    return even ? append_int8_kernel<T, true> : append_int8_kernel<T, false>;
   };
   auto kern = dtype == VFL_DTYPE_F32 ? pick(float()) : pick(__nv_bfloat16());
-  kern<<<(unsigned)ctas, threads, 0, s>>>(p);
-  return cuda_status(cudaGetLastError(), "reshape_and_cache_int8 launch");
+  if (p.window == 1) {
+    kern<<<(unsigned)ctas, threads, 0, s>>>(p);
+    return cuda_status(cudaGetLastError(), "reshape_and_cache_int8 launch");
+  }
+  const int64_t shares = ceil_div(num_tokens, (int64_t)(kRunsPerCta * kRunsCluster));
+  append_int8_runs_kernel<<<(unsigned)(shares * kRunsCluster), kRunsThreads, 0, s>>>(p);
+  st = cuda_status(cudaGetLastError(), "reshape_and_cache_int8 launch of its runs");
+  if (st) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, p), "reshape_and_cache_int8 launch");
 }
 
 int vfl_gather_kv_int8(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
