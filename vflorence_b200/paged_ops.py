@@ -769,7 +769,9 @@ def attention_with_kv_cache_int8(query: torch.Tensor, k_cache: torch.Tensor, v_c
     """``attention_with_kv_cache`` over an 8-bit cache (``reshape_and_cache_int8``): ``output =
     softmax(scale * q K^T) V`` per request over its paged tokens. Queries and output are float32
     or bfloat16; query head h reads K/V head ``h // (num_heads // num_kv_heads)``. Rows that see
-    no token are zeros. ``query_start_loc``, ``seq_lens`` and ``block_table`` may be host tensors."""
+    no token are zeros. A query element is held to 2^-23 (float32: 2^-31) of twice its row's largest, a
+    softmax weight to 11 (22) bits and 2^-32 of the largest. ``query_start_loc``, ``seq_lens`` and
+    ``block_table`` may be host tensors."""
     plan = plan_of_int8(scheduler_metadata)
     dev, n, h, bs, d = _int8_cache_checks(k_cache, v_cache, k_scale, v_scale)
     _require_cuda("query", query, dev)
