@@ -422,9 +422,10 @@ int vfl_plan_attention_int8_shape(vfl_attention_int8_plan* plan, int warps, int 
 /* As vfl_attention_with_kv_cache, over the 8-bit cache. Query head h reads K/V head
  * h / (num_heads / num_kv_heads). Sums, softmax statistics and the output before its last
  * rounding are float32; a query element is held to 2^-23 (float32: 2^-31) of twice its row's largest,
- * a softmax weight to 11 (22) bits and 2^-32 of the largest. V scales below 2^-100, and those 2^90 times smaller than another of the
- * context, may count as up to that much; so do scales of 0, whose blocks' codes are 0 (as the append
- * leaves them). A NaN scale makes the rows that see its block NaN. */
+ * a softmax weight to 11 (22) bits and 2^-32 of the largest. V scales below 2^-100, and those 2^90
+ * times smaller than another of the context, may count as up to that much; so do scales of 0, whose
+ * blocks' codes are 0 (as the append leaves them). A NaN scale makes the rows that see its block
+ * NaN. */
 int vfl_attention_with_kv_cache_int8(const vfl_attention_int8_plan* plan, const void* query,
                                      int64_t query_token_stride, const void* k_cache,
                                      const void* v_cache, const float* k_scale,
